@@ -469,6 +469,59 @@ int marl_ppo_apply(const MarlPpoApply *a, void *stream);
 int marl_fill_noise(const MarlEnvParams *p, const MarlEnvState *s, uint64_t seed,
                     uint64_t env_offset, double *noise, void *stream);
 
+/* ---- operators of a residual policy trunk and of the draw from its head ----------------------------------------------
+ * Rows of float32, bfloat16 or float16 (one type per call); `rows` is the product of all leading dimensions, ld_* are row
+ * strides in elements (>= the row length; the elements of a row are adjacent).  Any alignment of rows and any row length
+ * is taken; 16-byte aligned rows of a multiple of 16 bytes are the fast ones.  Nothing is allocated, nothing synchronises,
+ * no state is kept between calls; a workspace belongs to the call until it has run on its stream. */
+enum { MARL_F32 = 0, MARL_BF16 = 1, MARL_F16 = 2 };
+enum { MARL_ACT_SILU = 0, MARL_ACT_GELU = 1, MARL_ACT_RELU = 2, MARL_ACT_SIGMOID = 3 };      /* GELU: a Phi(a), by erf */
+enum { MARL_NORM_RMS = 0, MARL_NORM_LAYER = 1 };
+#define MARL_MAX_NORM_WIDTH 16384
+#define MARL_MAX_CHOICES (1 << 20)
+
+/* y[t][j] = act(a[t][j]) b[t][j],  a = x w_gate^T,  b = x w_up^T;  x [rows][d], weights [h][d], y [rows][h] contiguous.
+ * a, b: both NULL, or [rows][h] contiguous buffers that receive a and b for the backward call. */
+int marl_gated_forward(int32_t dtype, int32_t act, int64_t rows, int32_t d, int32_t h, const void *x, int64_t ldx,
+                       const void *w_gate, int64_t ld_gate, const void *w_up, int64_t ld_up, void *y, void *a, void *b,
+                       void *stream);
+/* dx [rows][d] (or NULL), dw_gate and dw_up [h][d] (or both NULL), all contiguous, from gy [rows][h] and the a, b of the
+ * forward call.  workspace: 16-byte aligned, marl_gated_workspace_bytes (0 for sizes the calls refuse). */
+size_t marl_gated_workspace_bytes(int32_t dtype, int64_t rows, int32_t d, int32_t h);
+int marl_gated_backward(int32_t dtype, int32_t act, int64_t rows, int32_t d, int32_t h, const void *x, int64_t ldx,
+                        const void *w_gate, int64_t ld_gate, const void *w_up, int64_t ld_up, const void *a, const void *b,
+                        const void *gy, int64_t ld_gy, void *dx, void *dw_gate, void *dw_up, void *workspace, void *stream);
+
+/* y = scale x + gate N(block; w_post),  n = N(y; w_pre), with N(v; w) = w (v - mean(v)) / sqrt(var(v) + eps) (MARL_NORM_LAYER)
+ * or w v / sqrt(mean(v^2) + eps) (MARL_NORM_RMS).  gate: NULL, one row of d (ld_gate = 0) or [rows][d].  y, n contiguous.
+ * stats: NULL or float [rows][4], 16-byte aligned, for the backward call.  d up to MARL_MAX_NORM_WIDTH. */
+int marl_residual_norm(int32_t dtype, int32_t kind, int64_t rows, int32_t d, const void *x, int64_t ldx, const void *block,
+                       int64_t ld_block, const void *w_post, const void *w_pre, const void *gate, int64_t ld_gate,
+                       float scale, float eps, void *y, void *n, float *stats, void *stream);
+/* Gradients from gy and gn (either may be NULL: zero): dx, dblock [rows][d], dw_post, dw_pre [d], dgate (shaped like gate,
+ * given exactly when gate is), all contiguous.  workspace: 16-byte aligned, marl_residual_norm_workspace_bytes. */
+size_t marl_residual_norm_workspace_bytes(int32_t d);
+int marl_residual_norm_backward(int32_t dtype, int32_t kind, int64_t rows, int32_t d, const void *y, const void *block,
+                                int64_t ld_block, const void *w_post, const void *w_pre, const void *gate, int64_t ld_gate,
+                                const float *stats, const void *gy, int64_t ld_gy, const void *gn, int64_t ld_gn, float scale,
+                                void *dx, void *dblock, void *dw_post, void *dw_pre, void *dgate, void *workspace, void *stream);
+
+/* y[r][j] = x[r][j] / (1 - p') where draw >= p', else 0;  p' = p rounded to a multiple of 2^-16, draw = 16 bits of
+ * Philox4x32-10 with counter (j / 8, 6, keys[r] low, keys[r] high) and key = seed: word (j % 8) / 2, low half first.
+ * keys NULL: the row number.  y [rows][d] contiguous.  The gradient is the same call on gy. */
+int marl_keyed_dropout(int32_t dtype, int64_t rows, int32_t d, const void *x, int64_t ldx, void *y, const int64_t *keys,
+                       double p, uint64_t seed, void *stream);
+
+/* One index per row of logits [rows][V] (V up to MARL_MAX_CHOICES): temperature (0: the first largest logit), top_k
+ * (0: off), top_p (1: off), min_p (0: off), in that order, then the first index, in index order, whose running weight
+ * exceeds u times the sum; log_prob is that index's log-probability among what was kept.  Equal logits: lower index
+ * first.  settings: NULL, or float [rows][4] = temperature, top_k, top_p, min_p of every row instead of the four scalars
+ * (out-of-range values there turn the filter off; temperature <= 0 is 0).  NaN logits count as -inf; a row without any
+ * other gives index -1 and log_prob -inf.  The result is a function of the row alone (no order of adding enters). */
+int marl_sample_logits(int32_t dtype, int64_t rows, int32_t V, const void *logits, int64_t ld, const float *u,
+                       float temperature, int32_t top_k, float top_p, float min_p, const float *settings, int64_t *index,
+                       float *log_prob, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

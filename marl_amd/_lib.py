@@ -23,10 +23,16 @@ STAGE_GENERAL_RESET = 4
 LAMBDA2_DIRECT, LAMBDA2_LANCZOS = 0x100, 0x200
 LAMBDA2_TEST_FEW_STEPS = 0x400        # testing: the bit-row Lanczos iteration gives up after 24 steps
 
+F32, BF16, F16 = 0, 1, 2
+ACTS = {"silu": 0, "gelu": 1, "relu": 2, "sigmoid": 3}
+NORMS = {"rms": 0, "layer": 1}
+MAX_NORM_WIDTH, MAX_CHOICES = 16384, 1 << 20
+
 MARL_OK, MARL_EINVAL, MARL_EUNSUPPORTED, MARL_EHIP, MARL_ETOOBIG = 0, -1, -2, -3, -4
 STATIC_SCRATCH_BYTES = 32 << 20
 
 _pd, _pf, _pi, _pu8, _pu32 = (C.c_void_p,) * 5   # device pointers travel as integers
+_p, _i32, _i64 = C.c_void_p, C.c_int32, C.c_int64
 
 
 class MarlEnvParams(C.Structure):
@@ -156,6 +162,17 @@ SYMBOLS = {
     "marl_ppo_apply": (C.c_int, [C.POINTER(MarlPpoApply), C.c_void_p]),
     "marl_fill_noise": (C.c_int, [C.POINTER(MarlEnvParams), C.POINTER(MarlEnvState), C.c_uint64, C.c_uint64,
                                   _pd, C.c_void_p]),
+    "marl_gated_forward": (C.c_int, [_i32, _i32, _i64, _i32, _i32, _p, _i64, _p, _i64, _p, _i64, _p, _p, _p, _p]),
+    "marl_gated_workspace_bytes": (C.c_size_t, [_i32, _i64, _i32, _i32]),
+    "marl_gated_backward": (C.c_int, [_i32, _i32, _i64, _i32, _i32, _p, _i64, _p, _i64, _p, _i64, _p, _p, _p, _i64, _p, _p, _p,
+                                      _p, _p]),
+    "marl_residual_norm": (C.c_int, [_i32, _i32, _i64, _i32, _p, _i64, _p, _i64, _p, _p, _p, _i64, C.c_float, C.c_float, _p, _p,
+                                     _p, _p]),
+    "marl_residual_norm_workspace_bytes": (C.c_size_t, [_i32]),
+    "marl_residual_norm_backward": (C.c_int, [_i32, _i32, _i64, _i32, _p, _p, _i64, _p, _p, _p, _i64, _p, _p, _i64, _p, _i64,
+                                              C.c_float, _p, _p, _p, _p, _p, _p, _p]),
+    "marl_keyed_dropout": (C.c_int, [_i32, _i64, _i32, _p, _i64, _p, _p, C.c_double, C.c_uint64, _p]),
+    "marl_sample_logits": (C.c_int, [_i32, _i64, _i32, _p, _i64, _p, C.c_float, _i32, C.c_float, C.c_float, _p, _p, _p, _p]),
 }
 
 _lib = None

@@ -42,6 +42,7 @@ __device__ __forceinline__ double u01(uint32_t hi, uint32_t lo) {   // (0,1), 53
     return ((double)(v & ((1ull << 53) - 1)) + 0.5) * (1.0 / 9007199254740992.0);
 }
 // Stream ids, mixed into the second counter word: one per consumer, so that no two draws share a counter.
-enum { STREAM_NOISE = 1, STREAM_RESET_ENEMY = 2, STREAM_RESET_JAMMER = 3, STREAM_RESET_ENV = 4, STREAM_POLICY = 5 };
+enum { STREAM_NOISE = 1, STREAM_RESET_ENEMY = 2, STREAM_RESET_JAMMER = 3, STREAM_RESET_ENV = 4, STREAM_POLICY = 5,
+       STREAM_DROPOUT = 6 };
 }  // namespace marl_rng
 #endif

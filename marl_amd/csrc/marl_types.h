@@ -1,0 +1,55 @@
+// Element types of the trunk operators (marl_gated.hip, marl_norm.hip, marl_dropout.hip, marl_sample.hip): float32,
+// bfloat16 and float16 in memory, float32 in registers; 16-byte chunks that need no more than element alignment.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "marl_env.h"
+
+namespace marl_types {
+
+typedef __bf16 bf16;
+typedef _Float16 f16;
+
+template <typename T> struct Chunk { static constexpr int n = 16 / (int)sizeof(T); };        // elements of 16 bytes
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(bf16 v) { return (float)v; }
+__device__ __forceinline__ float to_f32(f16 v) { return (float)v; }
+template <typename T> __device__ __forceinline__ T from_f32(float v) { return (T)v; }      // to nearest, ties to even
+
+template <typename T> struct alignas(16) Vec { T e[Chunk<T>::n]; };
+
+// 16 bytes from an address aligned to one element only: the hardware takes any alignment in global memory, so this is
+// one load; the compiler must merely not assume more.
+template <typename T> __device__ __forceinline__ Vec<T> load_chunk(const T* p) {
+    Vec<T> v;
+    __builtin_memcpy(&v, __builtin_assume_aligned(p, sizeof(T)), 16);
+    return v;
+}
+template <typename T> __device__ __forceinline__ void store_chunk(T* p, const Vec<T>& v) {
+    __builtin_memcpy(__builtin_assume_aligned(p, sizeof(T)), &v, 16);
+}
+// `left` elements remain from p on: whole chunks in one access, the last one element by element (the rest reads as zero)
+template <typename T> __device__ __forceinline__ Vec<T> load_part(const T* p, int64_t left) {
+    constexpr int n = Chunk<T>::n;
+    if (left >= n) return load_chunk(p);
+    Vec<T> v;
+#pragma unroll
+    for (int i = 0; i < n; ++i) v.e[i] = i < left ? p[i] : (T)0.0f;
+    return v;
+}
+template <typename T> __device__ __forceinline__ void store_part(T* p, const Vec<T>& v, int64_t left) {
+    constexpr int n = Chunk<T>::n;
+    if (left >= n) { store_chunk(p, v); return; }
+#pragma unroll
+    for (int i = 0; i < n; ++i) if (i < left) p[i] = v.e[i];
+}
+
+}  // namespace marl_types
+
+// Calls FN<T>(...) for the element type of `dtype`
+#define MARL_BY_TYPE(dtype, FN, ...)                                  \
+    ((dtype) == MARL_F32 ? FN<float>(__VA_ARGS__)                     \
+     : (dtype) == MARL_BF16 ? FN<marl_types::bf16>(__VA_ARGS__)       \
+                            : FN<marl_types::f16>(__VA_ARGS__))
