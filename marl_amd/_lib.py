@@ -164,7 +164,7 @@ SYMBOLS = {
                                   _pd, C.c_void_p]),
     "marl_gated_forward": (C.c_int, [_i32, _i32, _i64, _i32, _i32, _p, _i64, _p, _i64, _p, _i64, _p, _p, _p, _p]),
     "marl_gated_workspace_bytes": (C.c_size_t, [_i32, _i64, _i32, _i32]),
-    "marl_gated_backward": (C.c_int, [_i32, _i32, _i64, _i32, _i32, _p, _i64, _p, _i64, _p, _i64, _p, _p, _p, _i64, _p, _p, _p,
+    "marl_gated_backward": (C.c_int, [_i32, _i64, _i32, _i32, _p, _i64, _p, _i64, _p, _i64, _p, _p, _p, _i64, _p, _p, _p,
                                       _p, _p]),
     "marl_residual_norm": (C.c_int, [_i32, _i32, _i64, _i32, _p, _i64, _p, _i64, _p, _p, _p, _i64, C.c_float, C.c_float, _p, _p,
                                      _p, _p]),
@@ -198,6 +198,26 @@ def load():
         fn.argtypes = args
     _lib = lib
     return lib
+
+
+_torch_loaded = False
+
+
+def load_torch():
+    """Register the trunk operators (torch.ops.marl_amd.gated_linear, residual_norm, keyed_dropout, sample_logits) and bind
+    them to the library that load() uses; raise if either has not been built."""
+    global _torch_loaded
+    if _torch_loaded:
+        return
+    load()
+    path = os.path.join(_HERE, "libmarl_torch.so")
+    if not os.path.exists(path):
+        raise MarlError(f"{path} not found: build it with `python -c 'import __graft_entry__ as g; g.build()'`")
+    import torch
+    torch.ops.load_library(path)
+    if C.CDLL(path).marl_torch_bind(os.path.abspath(LIB_PATH).encode()) != 0:
+        raise MarlError(f"{LIB_PATH} lacks an entry point of the trunk operators: build it again")
+    _torch_loaded = True
 
 
 def check(code, what=""):

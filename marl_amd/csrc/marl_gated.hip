@@ -1,5 +1,5 @@
 // Gated projections  y = act(a) * b,  a = x Wg^T, b = x Wu^T  (x [T, d], Wg and Wu [h, d]) and their gradients
-//     da = gy b act'(a),  db = gy act(a),  dx = da Wg + db Wu,  dWg = da^T x,  dWu = db^T x.
+//     da = gy p,  db = gy f,  f = act(a),  p = b act'(a),  dx = da Wg + db Wu,  dWg = da^T x,  dWu = db^T x.
 // All five contractions are one tiled product on the matrix cores, C[m][n] = sum_k A(m, k) B(n, k), in three settings:
 //     FWD   A = x (k contiguous), B = rows of Wg and Wu in alternating groups of 32, so that a lane holds a and b of the
 //           same (t, j) and the activation and the product happen in its registers
@@ -11,8 +11,8 @@
 // no transposed copy of a weight or a gradient is ever made.  Chunk positions are permuted within a row (tile_* below) so
 // that the lanes of one LDS access fall on different banks.
 // 16-bit types: v_mfma_f32_32x32x16 with float32 accumulators; float32: v_mfma_f32_32x32x2.  da and db are rounded to
-// the element type, once, because they are matrix operands; a and b are kept in it between forward and backward (T h
-// elements each, against 4 T d h operations for computing them again).
+// the element type, once, because they are matrix operands; f and p are kept in it between forward and backward (T h
+// elements each, against 4 T d h operations for computing a and b again).
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -70,11 +70,6 @@ template <int ACT, bool FAST> __device__ __forceinline__ void act_both(float a, 
         else { f = a * s; df = s * (1.0f + a * (1.0f - s)); }
     }
 }
-template <int ACT, bool FAST> __device__ __forceinline__ float act_of(float a) {
-    float f, df;
-    act_both<ACT, FAST>(a, f, df);
-    return f;
-}
 template <class F> __device__ __forceinline__ void by_act(int act, F&& f) {
     switch (act) {
         case MARL_ACT_SILU: f(std::integral_constant<int, MARL_ACT_SILU>{}); break;
@@ -95,11 +90,21 @@ struct ProductArgs {
     int64_t h;
     int64_t k_chunk;          // k range of one z slice, a multiple of the step
     void *out0, *out1;        // FWD: y; DX: dx; DW: dWg, dWu
-    void *save_a, *save_b;    // FWD
+    void *save_f, *save_p;    // FWD: NULL, or what backward needs
     float* partial;           // [slices][M][N] when the k range is split
     int act;
     int tiles_m, tiles_n;
 };
+
+template <typename T, int ACT> __device__ __forceinline__ void gate_out(const ProductArgs& args, int64_t at, float a, float b) {
+    float f, df;
+    act_both<ACT, sizeof(T) == 2>(a, f, df);
+    ((T*)args.out0)[at] = from_f32<T>(f * b);
+    if (args.save_f) {
+        ((T*)args.save_f)[at] = from_f32<T>(f);
+        ((T*)args.save_p)[at] = from_f32<T>(b * df);
+    }
+}
 
 // position of chunk c in row r of a tile with k along the row (8 chunks a row)
 __device__ __forceinline__ int tile_k_along(int r, int c) { return c ^ (r & 7); }
@@ -151,21 +156,39 @@ struct Tile {
             return (const T*)o.p0 + rr * o.ld0;
         }
     }
-    // direct global -> LDS: every k of the step exists, chunks are aligned and whole; rows and columns beyond the edge
-    // repeat the last ones (their results are never stored)
-    static __device__ __forceinline__ void load_direct(const ProductArgs& a, int64_t row0, int64_t rows, int64_t k0, char* lds) {
-        const int tid = threadIdx.x;
+    // The thread's chunks at k = 0, found once: a step then adds one offset to all of them.  DX's B reads the second
+    // weight from k = h on: its chunks at k = h.
+    struct Pointers {
+        const T* at[PER];
+        const T* at2[MODE == DX && IS_B ? PER : 1];
+    };
+    static __device__ __forceinline__ void pointers(const ProductArgs& a, int64_t row0, int64_t rows, Pointers& p) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int q = i * THREADS + tid;
             int r, e;
-            place(q, r, e);
-            int64_t row;
-            const T* p = row_ptr(a, row0, k0, r, row, rows);
-            int64_t col = (ACROSS ? row0 : k0) + e;
-            if constexpr (ACROSS) col = col < rows ? col : rows - CE;
-            char* dst = lds + (size_t)(i * THREADS + (tid & ~63)) * 16;
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(p + col),
+            place(i * THREADS + (int)threadIdx.x, r, e);
+            if constexpr (ACROSS) {       // columns beyond the edge repeat the last chunk (their results are never stored)
+                const int64_t col = row0 + e < rows ? row0 + e : rows - CE;
+                const Operand& o = IS_B ? a.B : a.A;
+                p.at[i] = (const T*)o.p0 + r * o.ld0 + col;
+                if constexpr (MODE == DX) p.at2[i] = (const T*)o.p1 + r * o.ld1 + col;
+            } else {                      // rows beyond the edge repeat the last one
+                int64_t row;
+                p.at[i] = row_ptr(a, row0, 0, r, row, rows) + e;
+            }
+        }
+    }
+    // direct global -> LDS: every k of the step exists (DX: on one side of h), chunks are aligned and whole
+    static __device__ __forceinline__ void load_direct(const ProductArgs& a, const Pointers& p, int64_t k0, char* lds) {
+        const Operand& o = IS_B ? a.B : a.A;
+        const bool second = MODE == DX && IS_B && k0 >= a.h;
+        const int64_t step = !ACROSS ? k0 : second ? (k0 - a.h) * o.ld1 : k0 * o.ld0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const T* src = p.at[i];
+            if constexpr (MODE == DX && IS_B) src = second ? p.at2[i] : src;
+            char* dst = lds + (size_t)(i * THREADS + (threadIdx.x & ~63)) * 16;
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + step),
                                              (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
         }
     }
@@ -255,12 +278,16 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
     const int steps = (int)((k_end - k_begin + BK - 1) / BK);
     floatx16 acc[MI][NI] = {};
     Vec<T> va[TA::PER], vb[TB::PER];
+    typename TA::Pointers pa;
+    typename TB::Pointers pb;
+    if (DIRECT) { TA::pointers(args, m0, args.M, pa); TB::pointers(args, n0, args.N, pb); }
 
-    auto fetch = [&](int s, char* buf) {       // DIRECT: into `buf` (a ragged last step through registers); else into registers
+    // Step s into `buf`: direct loads, or (a ragged step; every step if !DIRECT) into registers, which commit() stores.
+    auto fetch = [&](int s, char* buf) {
         const int64_t k0 = k_begin + (int64_t)s * BK;
-        if (DIRECT && k0 + BK <= k_end) {
-            TA::load_direct(args, m0, args.M, k0, buf);
-            TB::load_direct(args, n0, args.N, k0, buf + A_BYTES);
+        if (DIRECT && k0 + BK <= k_end && (MODE != DX || k0 + BK <= args.h || k0 >= args.h)) {
+            TA::load_direct(args, pa, k0, buf);
+            TB::load_direct(args, pb, k0, buf + A_BYTES);
         } else {
             TA::load_masked(args, m0, args.M, k0, k_end, va);
             TB::load_masked(args, n0, args.N, k0, k_end, vb);
@@ -270,27 +297,38 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
     auto commit = [&](char* buf) {
         if (!DIRECT) { TA::store_lds(buf, va); TB::store_lds(buf + A_BYTES, vb); }
     };
+    typename Frag<T>::type fa[2][MI], fb[2][NI];
+    auto read = [&](const char* buf, int ks, int to) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i) fa[to][i] = TA::frag(buf, wm * (BM / WM) + 32 * i, ks, lane);
+#pragma unroll
+        for (int j = 0; j < NI; ++j) fb[to][j] = TB::frag(buf + A_BYTES, wn * (BN / WN) + 32 * j, ks, lane);
+    };
+    auto multiply = [&](int from) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < NI; ++j) acc[i][j] = mma(T(), fa[from][i], fb[from][j], acc[i][j]);
+    };
+    // Operands are read one k step ahead of their use, and the barrier between two buffers stands before the last
+    // k step's products, which cover the first reads of the new buffer.
     fetch(0, lds);
     commit(lds);
     __syncthreads();
+    read(lds, 0, 0);
     for (int s = 0; s < steps; ++s) {
         char* cur = lds + (s & 1) * BUF;
         char* nxt = lds + ((s + 1) & 1) * BUF;
         if (s + 1 < steps) fetch(s + 1, nxt);
 #pragma unroll
-        for (int ks = 0; ks < KSTEPS; ++ks) {
-            typename Frag<T>::type fa[MI], fb[NI];
-#pragma unroll
-            for (int i = 0; i < MI; ++i) fa[i] = TA::frag(cur, wm * (BM / WM) + 32 * i, ks, lane);
-#pragma unroll
-            for (int j = 0; j < NI; ++j) fb[j] = TB::frag(cur + A_BYTES, wn * (BN / WN) + 32 * j, ks, lane);
-#pragma unroll
-            for (int i = 0; i < MI; ++i)
-#pragma unroll
-                for (int j = 0; j < NI; ++j) acc[i][j] = mma(T(), fa[i], fb[j], acc[i][j]);
+        for (int ks = 0; ks + 1 < KSTEPS; ++ks) {
+            read(cur, ks + 1, (ks + 1) & 1);
+            multiply(ks & 1);
         }
         if (s + 1 < steps) commit(nxt);
         __syncthreads();
+        if (s + 1 < steps) read(nxt, 0, 0);
+        multiply((KSTEPS - 1) & 1);
     }
     // register v of a lane: row 8 (v / 4) + 4 (lane / 32) + v % 4, column lane % 32
     const int hl = lane >> 5, col = lane & 31;
@@ -305,13 +343,7 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
                 for (int v = 0; v < 16; ++v) {
                     const int64_t m = m0 + wm * (BM / WM) + 32 * i + 8 * (v / 4) + 4 * hl + v % 4;
                     if (m >= args.M) continue;
-                    const float a = acc[i][0][v], b = acc[i][1][v];
-                    const int64_t at = m * args.N + n;
-                    ((T*)args.out0)[at] = from_f32<T>(act_of<ACT, sizeof(T) == 2>(a) * b);
-                    if (args.save_a) {
-                        ((T*)args.save_a)[at] = from_f32<T>(a);
-                        ((T*)args.save_b)[at] = from_f32<T>(b);
-                    }
+                    gate_out<T, ACT>(args, m * args.N + n, acc[i][0][v], acc[i][1][v]);
                 }
         });
     } else {
@@ -414,41 +446,31 @@ __global__ __launch_bounds__(512) void gated_few_rows_kernel(const ProductArgs a
                 a += part[(((w * MT + i) * 2 + 0) * 16 + v) * 64 + lane];
                 b += part[(((w * MT + i) * 2 + 1) * 16 + v) * 64 + lane];
             }
-            const int64_t at = t * args.N + j;
-            ((T*)args.out0)[at] = from_f32<T>(act_of<ACT, sizeof(T) == 2>(a) * b);
-            if (args.save_a) {
-                ((T*)args.save_a)[at] = from_f32<T>(a);
-                ((T*)args.save_b)[at] = from_f32<T>(b);
-            }
+            gate_out<T, ACT>(args, t * args.N + j, a, b);
         }
     });
 }
 
-// [da | db] of every row: bandwidth (three reads, two writes of T h)
+// [da | db] = [gy p | gy f] of every row: bandwidth (three reads, two writes of T h)
 template <typename T>
-__global__ __launch_bounds__(256) void gated_da_db_kernel(const T* __restrict__ a, const T* __restrict__ b, const T* __restrict__ gy, int64_t ldgy,
-                                                           T* __restrict__ dab, int64_t rows, int64_t h, int act) {
+__global__ __launch_bounds__(256) void gated_da_db_kernel(const T* __restrict__ f, const T* __restrict__ p, const T* __restrict__ gy, int64_t ldgy,
+                                                           T* __restrict__ dab, int64_t rows, int64_t h) {
     constexpr int CE = Chunk<T>::n;
     const int64_t per = (h + CE - 1) / CE;
-    by_act(act, [&](auto kind) {
-        constexpr int ACT = decltype(kind)::value;
-        for (int64_t t = blockIdx.y; t < rows; t += gridDim.y)
-            for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < per; q += (int64_t)gridDim.x * 256) {
-                const int64_t c = q * CE, left = h - c;
-                const Vec<T> va = load_part(a + t * h + c, left), vb = load_part(b + t * h + c, left), vg = load_part(gy + t * ldgy + c, left);
-                Vec<T> da, db;
+    for (int64_t t = blockIdx.y; t < rows; t += gridDim.y)
+        for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < per; q += (int64_t)gridDim.x * 256) {
+            const int64_t c = q * CE, left = h - c;
+            const Vec<T> vf = load_part(f + t * h + c, left), vp = load_part(p + t * h + c, left), vg = load_part(gy + t * ldgy + c, left);
+            Vec<T> da, db;
 #pragma unroll
-                for (int i = 0; i < CE; ++i) {
-                    float f, df;
-                    act_both<ACT, sizeof(T) == 2>(to_f32(va.e[i]), f, df);
-                    const float g = to_f32(vg.e[i]);
-                    da.e[i] = from_f32<T>(g * to_f32(vb.e[i]) * df);
-                    db.e[i] = from_f32<T>(g * f);
-                }
-                store_part(dab + t * 2 * h + c, da, left);
-                store_part(dab + t * 2 * h + h + c, db, left);
+            for (int i = 0; i < CE; ++i) {
+                const float g = to_f32(vg.e[i]);
+                da.e[i] = from_f32<T>(g * to_f32(vp.e[i]));
+                db.e[i] = from_f32<T>(g * to_f32(vf.e[i]));
             }
-    });
+            store_part(dab + t * 2 * h + c, da, left);
+            store_part(dab + t * 2 * h + h + c, db, left);
+        }
 }
 
 // -- host ------------------------------------------------------------------------------------------------------------
@@ -521,13 +543,13 @@ template <typename T, int MT> hipError_t launch_few_rows(const ProductArgs& a, h
 }
 
 template <typename T> int forward(int act, int64_t rows, int32_t d, int32_t h, const void* x, int64_t ldx, const void* wg, int64_t ldg,
-                                  const void* wu, int64_t ldu, void* y, void* a, void* b, hipStream_t stream) {
-    ProductArgs p = {};
-    p.A = {x, nullptr, ldx, 0};
-    p.B = {wg, wu, ldg, ldu};
-    p.M = rows; p.N = h; p.K = d; p.h = h;
-    p.out0 = y; p.save_a = a; p.save_b = b; p.act = act;
-    hipError_t err = rows <= 32 ? launch_few_rows<T, 1>(p, stream) : rows <= 64 ? launch_few_rows<T, 2>(p, stream) : launch_product<T, FWD>(p, nullptr, stream);
+                                  const void* wu, int64_t ldu, void* y, void* f, void* p, hipStream_t stream) {
+    ProductArgs a = {};
+    a.A = {x, nullptr, ldx, 0};
+    a.B = {wg, wu, ldg, ldu};
+    a.M = rows; a.N = h; a.K = d; a.h = h;
+    a.out0 = y; a.save_f = f; a.save_p = p; a.act = act;
+    hipError_t err = rows <= 32 ? launch_few_rows<T, 1>(a, stream) : rows <= 64 ? launch_few_rows<T, 2>(a, stream) : launch_product<T, FWD>(a, nullptr, stream);
     if (err == hipSuccess) return MARL_OK;
     marl_note_hip_error((int)err);
     return MARL_EHIP;
@@ -541,28 +563,28 @@ template <typename T> size_t workspace(int64_t rows, int32_t d, int32_t h) {
     return (size_t)(round_256(rows * 2 * h * (int64_t)sizeof(T)) + (sx > sw ? sx : sw) * (int64_t)sizeof(float));
 }
 
-template <typename T> int backward(int act, int64_t rows, int32_t d, int32_t h, const void* x, int64_t ldx, const void* wg, int64_t ldg,
-                                   const void* wu, int64_t ldu, const void* a, const void* b, const void* gy, int64_t ldgy, void* dx,
+template <typename T> int backward(int64_t rows, int32_t d, int32_t h, const void* x, int64_t ldx, const void* wg, int64_t ldg,
+                                   const void* wu, int64_t ldu, const void* f, const void* p, const void* gy, int64_t ldgy, void* dx,
                                    void* dwg, void* dwu, void* ws, hipStream_t stream) {
     T* dab = (T*)ws;
     float* partial = (float*)((char*)ws + round_256(rows * 2 * h * (int64_t)sizeof(T)));
     const int64_t per = (h + Chunk<T>::n - 1) / Chunk<T>::n;
     hipLaunchKernelGGL(gated_da_db_kernel<T>, dim3((unsigned)((per + 255) / 256), (unsigned)(rows < 65535 ? rows : 65535)), dim3(256), 0, stream,
-                       (const T*)a, (const T*)b, (const T*)gy, ldgy, dab, rows, (int64_t)h, act);
+                       (const T*)f, (const T*)p, (const T*)gy, ldgy, dab, rows, (int64_t)h);
     hipError_t err = hipGetLastError();
     if (err == hipSuccess && dx) {
-        ProductArgs p = {};
-        p.A = {dab, nullptr, 2 * (int64_t)h, 0};
-        p.B = {wg, wu, ldg, ldu};
-        p.M = rows; p.N = d; p.K = 2 * (int64_t)h; p.h = h; p.out0 = dx;
-        err = launch_product<T, DX>(p, partial, stream);
+        ProductArgs a = {};
+        a.A = {dab, nullptr, 2 * (int64_t)h, 0};
+        a.B = {wg, wu, ldg, ldu};
+        a.M = rows; a.N = d; a.K = 2 * (int64_t)h; a.h = h; a.out0 = dx;
+        err = launch_product<T, DX>(a, partial, stream);
     }
     if (err == hipSuccess && dwg) {
-        ProductArgs p = {};
-        p.A = {dab, nullptr, 2 * (int64_t)h, 0};
-        p.B = {x, nullptr, ldx, 0};
-        p.M = 2 * (int64_t)h; p.N = d; p.K = rows; p.h = h; p.out0 = dwg; p.out1 = dwu;
-        err = launch_product<T, DW>(p, partial, stream);
+        ProductArgs a = {};
+        a.A = {dab, nullptr, 2 * (int64_t)h, 0};
+        a.B = {x, nullptr, ldx, 0};
+        a.M = 2 * (int64_t)h; a.N = d; a.K = rows; a.h = h; a.out0 = dwg; a.out1 = dwu;
+        err = launch_product<T, DW>(a, partial, stream);
     }
     if (err == hipSuccess) return MARL_OK;
     marl_note_hip_error((int)err);
@@ -583,13 +605,13 @@ int check_sizes(int32_t dtype, int32_t act, int64_t rows, int32_t d, int32_t h) 
 extern "C" {
 
 int marl_gated_forward(int32_t dtype, int32_t act, int64_t rows, int32_t d, int32_t h, const void* x, int64_t ldx, const void* w_gate,
-                       int64_t ld_gate, const void* w_up, int64_t ld_up, void* y, void* a, void* b, void* stream) {
+                       int64_t ld_gate, const void* w_up, int64_t ld_up, void* y, void* f, void* p, void* stream) {
     const int rc = check_sizes(dtype, act, rows, d, h);
     if (rc != MARL_OK) return rc;
-    if (!x || !w_gate || !w_up || !y || (a == nullptr) != (b == nullptr)) return MARL_EINVAL;
+    if (!x || !w_gate || !w_up || !y || (f == nullptr) != (p == nullptr)) return MARL_EINVAL;
     if (ldx < d && rows > 1) return MARL_EINVAL;
     if ((ld_gate < d || ld_up < d) && h > 1) return MARL_EINVAL;
-    return MARL_BY_TYPE(dtype, forward, act, rows, d, h, x, ldx, w_gate, ld_gate, w_up, ld_up, y, a, b, (hipStream_t)stream);
+    return MARL_BY_TYPE(dtype, forward, act, rows, d, h, x, ldx, w_gate, ld_gate, w_up, ld_up, y, f, p, (hipStream_t)stream);
 }
 
 size_t marl_gated_workspace_bytes(int32_t dtype, int64_t rows, int32_t d, int32_t h) {
@@ -597,15 +619,15 @@ size_t marl_gated_workspace_bytes(int32_t dtype, int64_t rows, int32_t d, int32_
     return MARL_BY_TYPE(dtype, workspace, rows, d, h);
 }
 
-int marl_gated_backward(int32_t dtype, int32_t act, int64_t rows, int32_t d, int32_t h, const void* x, int64_t ldx, const void* w_gate,
-                        int64_t ld_gate, const void* w_up, int64_t ld_up, const void* a, const void* b, const void* gy, int64_t ld_gy,
+int marl_gated_backward(int32_t dtype, int64_t rows, int32_t d, int32_t h, const void* x, int64_t ldx, const void* w_gate,
+                        int64_t ld_gate, const void* w_up, int64_t ld_up, const void* f, const void* p, const void* gy, int64_t ld_gy,
                         void* dx, void* dw_gate, void* dw_up, void* workspace_, void* stream) {
-    const int rc = check_sizes(dtype, act, rows, d, h);
+    const int rc = check_sizes(dtype, MARL_ACT_SILU, rows, d, h);
     if (rc != MARL_OK) return rc;
-    if (!x || !w_gate || !w_up || !a || !b || !gy || !workspace_ || ((uintptr_t)workspace_ & 15) || (dw_gate == nullptr) != (dw_up == nullptr)) return MARL_EINVAL;
+    if (!x || !w_gate || !w_up || !f || !p || !gy || !workspace_ || ((uintptr_t)workspace_ & 15) || (dw_gate == nullptr) != (dw_up == nullptr)) return MARL_EINVAL;
     if ((ldx < d || ld_gy < h) && rows > 1) return MARL_EINVAL;
     if ((ld_gate < d || ld_up < d) && h > 1) return MARL_EINVAL;
-    return MARL_BY_TYPE(dtype, backward, act, rows, d, h, x, ldx, w_gate, ld_gate, w_up, ld_up, a, b, gy, ld_gy, dx, dw_gate, dw_up, workspace_,
+    return MARL_BY_TYPE(dtype, backward, rows, d, h, x, ldx, w_gate, ld_gate, w_up, ld_up, f, p, gy, ld_gy, dx, dw_gate, dw_up, workspace_,
                         (hipStream_t)stream);
 }
 

@@ -2,7 +2,7 @@
 
 Tolerances are bounds, worked out per element before the comparison: a result rounded to type t is off by at most half a
 step (eps(t) / 2 of its value); a float32 sum of n terms by at most (n + 8) 2^-24 of the sum of their magnitudes; values
-kept in t between forward and backward (a, b, da, db, y) by half a step each, carried through the formulas."""
+kept in t between forward and backward (f, p, y) and matrix operands (da, db) by half a step each, carried through the formulas."""
 import numpy as np
 import pytest
 import torch
@@ -63,15 +63,15 @@ def gated_oracle(x, wg, wu, gy, kind):
     ef = dmax * ea + 2.0 ** -20 * (1 + a.abs())
     y = f * b
     ty = e * y.abs() + (b.abs() * ef + f.abs() * eb + ef * eb) * 1.01 + 2 * U * y.abs() + tiny(dt)
-    # backward works from a and b rounded to the type
-    ea, eb = ea + e * a.abs() + tiny(dt), eb + e * b.abs() + tiny(dt)
+    # backward works from f = act(a) and p = b act'(a), rounded to the type
     edf = d2max * ea + 2.0 ** -20 * (1 + a.abs())
     if kind == "relu":
         edf = edf + (a.abs() <= ea).double()                         # the step of the derivative at 0
-    ef = dmax * ea + 2.0 ** -20 * (1 + a.abs())
+    p = b * df
+    ep = b.abs() * edf + df.abs() * eb + eb * edf + (e + 2 * U) * p.abs() + tiny(dt)
+    ef = ef + e * f.abs() + tiny(dt)
     da, db = gy * b * df, gy * f
-    eda = gy.abs() * (b.abs() * edf + df.abs() * eb + eb * edf) * 1.01
-    edb = gy.abs() * ef * 1.01
+    eda, edb = gy.abs() * ep * 1.01, gy.abs() * ef * 1.01
     eda, edb = eda + (e + 4 * U) * (da.abs() + eda) + tiny(dt), edb + (e + 4 * U) * (db.abs() + edb) + tiny(dt)
     dx, dwg, dwu = da @ wg + db @ wu, da.t() @ x, db.t() @ x
     n, T = 2 * wg.shape[0], x.shape[0]
@@ -89,7 +89,7 @@ def gated_check(T, d, h, dt, kind, seed=0, prepare=lambda t: t, name=""):
     xd, gd, ud = (prepare(t.cuda()).requires_grad_(True) for t in (x, wg, wu))
     y = ops.gated_linear(xd, gd, ud, kind)
     with torch.no_grad():
-        assert torch.equal(y, ops.gated_linear(xd, gd, ud, kind))                    # with and without kept a, b
+        assert torch.equal(y, ops.gated_linear(xd, gd, ud, kind))                    # with and without kept f, p
     grads = torch.autograd.grad(y, (xd, gd, ud), gy.cuda())
     for n_, g, w, t in zip(("y", "dx", "dw_gate", "dw_up"), (y,) + grads, want, tol):
         close(f"{name} {n_}", g, w, t)

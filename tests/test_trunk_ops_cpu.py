@@ -73,7 +73,7 @@ def test_entry_points_check_their_arguments():
         assert gf(**bad) == E, bad
     assert gf(rows=1 << 31) == U and gf(d=(1 << 24) + 1, ldx=1 << 25, ldg=1 << 25) == U
     gb = lambda rows=2, d=8, h=8, a=P, gy=P, ldgy=8, dx=P, dwg=P, dwu=P, ws=P: \
-        lib.marl_gated_backward(0, 0, rows, d, h, P, 8, P, 8, P, 8, a, P, gy, ldgy, dx, dwg, dwu, ws, None)
+        lib.marl_gated_backward(0, rows, d, h, P, 8, P, 8, P, 8, a, P, gy, ldgy, dx, dwg, dwu, ws, None)
     for bad in (dict(rows=0), dict(a=None), dict(gy=None), dict(ldgy=7), dict(dwu=None), dict(ws=None), dict(ws=P + 8)):
         assert gb(**bad) == E, bad
     assert lib.marl_gated_workspace_bytes(0, 0, 8, 8) == 0 and lib.marl_gated_workspace_bytes(1, 100, 8, 16) >= 100 * 32 * 2
