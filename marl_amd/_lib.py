@@ -162,8 +162,8 @@ SYMBOLS = {
     "marl_ppo_apply": (C.c_int, [C.POINTER(MarlPpoApply), C.c_void_p]),
     "marl_fill_noise": (C.c_int, [C.POINTER(MarlEnvParams), C.POINTER(MarlEnvState), C.c_uint64, C.c_uint64,
                                   _pd, C.c_void_p]),
-    "marl_gated_forward": (C.c_int, [_i32, _i32, _i64, _i32, _i32, _p, _i64, _p, _i64, _p, _i64, _p, _p, _p, _p]),
-    "marl_gated_workspace_bytes": (C.c_size_t, [_i32, _i64, _i32, _i32]),
+    "marl_gated_forward": (C.c_int, [_i32, _i32, _i64, _i32, _i32, _p, _i64, _p, _i64, _p, _i64, _p, _p, _p, _p, _p]),
+    "marl_gated_workspace_bytes": (C.c_size_t, [_i32, _i64, _i32, _i32, _p, _i64, _p, _i64, _p, _i64, _i32]),
     "marl_gated_backward": (C.c_int, [_i32, _i64, _i32, _i32, _p, _i64, _p, _i64, _p, _i64, _p, _p, _p, _i64, _p, _p, _p,
                                       _p, _p]),
     "marl_residual_norm": (C.c_int, [_i32, _i32, _i64, _i32, _p, _i64, _p, _i64, _p, _p, _p, _i64, C.c_float, C.c_float, _p, _p,

@@ -3,10 +3,13 @@
 // All five contractions are one tiled product on the matrix cores, C[m][n] = sum_k A(m, k) B(n, k), in three settings:
 //     FWD   A = x (k contiguous), B = rows of Wg and Wu in alternating groups of 32, so that a lane holds a and b of the
 //           same (t, j) and the activation and the product happen in its registers
-//     DX    A = [da | db] (k contiguous, 2h long), B = Wg then Wu with k along their rows
-//     DW    A = [da | db]^T, B = x^T, both with k along their rows; the 2h rows of C are dWg then dWu
-// Operands travel global -> LDS in 16-byte chunks (direct loads where every chunk is aligned and whole, through registers
-// otherwise), two buffers of 128 bytes of k per row.  Tiles with k along the row are read back with ds_read_b128, tiles
+//     DX    A = [da | db] (k contiguous), B = Wg then Wu with k across their rows
+//     DW    A = [da | db]^T, B = x^T, both with k across their rows; the 2h rows of C are dWg then dWu
+// Operands travel global -> LDS in 16-byte chunks by direct loads (a ragged last step of k through registers) into a ring
+// of five stages of 64 bytes of k per row: three stages are under way while one is multiplied, which covers the latency of
+// a miss in L2 (with two stages of 128 bytes the loop waited for memory half of its time), and the fifth place lets a wave
+// pass a barrier without waiting for its own LDS reads.  Operands whose rows are not
+// aligned to chunks are first copied to rows that are.  Tiles with k along the row are read back with ds_read_b128, tiles
 // with k across the rows with ds_read_b64_tr_b16 (a 4 x 16 transpose in the read; float32 reads its single elements), so
 // no transposed copy of a weight or a gradient is ever made.  Chunk positions are permuted within a row (tile_* below) so
 // that the lanes of one LDS access fall on different banks.
@@ -29,7 +32,8 @@ using namespace marl_types;
 using marl_net::floatx16;
 
 enum Mode { FWD, DX, DW };
-constexpr int ROW_BYTES = 128;               // bytes of k per tile row and step
+constexpr int ROW_BYTES = 64;                // bytes of k per tile row and stage
+constexpr int STAGES = 5, AHEAD = 3;         // places of the ring; stages under way while one is multiplied
 
 typedef short short4v __attribute__((ext_vector_type(4)));
 typedef short short8v __attribute__((ext_vector_type(8)));
@@ -81,14 +85,14 @@ template <class F> __device__ __forceinline__ void by_act(int act, F&& f) {
 
 // -- tiles -----------------------------------------------------------------------------------------------------------
 struct Operand {
-    const void *p0, *p1;      // p1: the second weight (FWD: odd groups of 32 rows, DX: k >= h)
+    const void *p0, *p1;      // p1: the second weight (FWD: odd groups of 32 rows, DX: the second pass over k)
     int64_t ld0, ld1;
 };
 struct ProductArgs {
     Operand A, B;
-    int64_t M, N, K;          // FWD: M = T, N = h, K = d.  DX: T, d, 2h.  DW: 2h, d, T.
-    int64_t h;
-    int64_t k_chunk;          // k range of one z slice, a multiple of the step
+    int64_t M, N, K;          // FWD: M = T, N = h, K = d.  DX: T, d, h, twice: for da and for db.  DW: 2 half, d, T.
+    int64_t h, half;          // backward: db stands `half` columns behind da (h rounded up to whole chunks)
+    int stages;               // stages of k in one slice
     void *out0, *out1;        // FWD: y; DX: dx; DW: dWg, dWu
     void *save_f, *save_p;    // FWD: NULL, or what backward needs
     float* partial;           // [slices][M][N] when the k range is split
@@ -96,27 +100,45 @@ struct ProductArgs {
     int tiles_m, tiles_n;
 };
 
-template <typename T, int ACT> __device__ __forceinline__ void gate_out(const ProductArgs& args, int64_t at, float a, float b) {
-    float f, df;
-    act_both<ACT, sizeof(T) == 2>(a, f, df);
-    ((T*)args.out0)[at] = from_f32<T>(f * b);
+// y, and f and p for backward, of `left` (at most a chunk) neighbouring columns from their a and b
+template <typename T, int ACT> __device__ __forceinline__ void gate_out(const ProductArgs& args, int64_t at, const float* a, const float* b, int64_t left) {
+    constexpr int CE = Chunk<T>::n;
+    Vec<T> y, vf, vp;
+#pragma unroll
+    for (int e = 0; e < CE; ++e) {
+        float f, df;
+        act_both<ACT, sizeof(T) == 2>(a[e], f, df);
+        y.e[e] = from_f32<T>(f * b[e]);
+        vf.e[e] = from_f32<T>(f);
+        vp.e[e] = from_f32<T>(b[e] * df);
+    }
+    store_part((T*)args.out0 + at, y, left);
     if (args.save_f) {
-        ((T*)args.save_f)[at] = from_f32<T>(f);
-        ((T*)args.save_p)[at] = from_f32<T>(b * df);
+        store_part((T*)args.save_f + at, vf, left);
+        store_part((T*)args.save_p + at, vp, left);
     }
 }
 
-// position of chunk c in row r of a tile with k along the row (8 chunks a row)
-__device__ __forceinline__ int tile_k_along(int r, int c) { return c ^ (r & 7); }
-// position of chunk c in k-row kr of a tile with k across the rows.  16-bit: pairs of chunks (the 16 elements one
-// transposing read takes from a row) are permuted by the four rows and the row octet that one access covers; float32:
+// position of chunk c in row r of a tile with k along the row (4 chunks a row): sixteen consecutive rows, read at one
+// chunk, cover all 64 banks
+__device__ __forceinline__ int tile_k_along(int r, int c) { return c ^ ((r >> 2) & 3); }
+// position of chunk c in k-row kr of a tile with k across the rows.  16-bit: a half wave's
+// transposing read takes 64 bytes (four chunks) from each of four consecutive rows, which go to different quarters of the banks; float32:
 // the two half waves read rows four apart, which go to different 128-byte halves.
 template <typename T> __device__ __forceinline__ int tile_k_across(int kr, int c) {
-    if constexpr (sizeof(T) == 2) return c ^ (((kr & 3) | (((kr >> 3) & 1) << 2)) << 1);
+    if constexpr (sizeof(T) == 2) return c ^ ((kr & 3) << 2);
     else return c ^ (((kr >> 2) & 1) << 3);
 }
 
 typedef __attribute__((address_space(3))) char lds_char;
+
+// 16 bytes per lane from `src` to LDS at `dst` (the same for the whole wave) + 16 lane.  In assembly because the compiler
+// makes every LDS read behind the builtin wait for all of these loads; here wait_loads() counts them.  The statement has no
+// output registers, and the wait on M0 is inside it.
+__device__ __forceinline__ void load_to_lds(const void* src, char* dst) {
+    const int at = __builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(lds_char*)dst);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(src) : "memory", "m0");
+}
 
 // One operand's tile: ROWS rows (m or n) by ROW_BYTES of k.  ACROSS: k runs across the rows of memory.
 template <typename T, int MODE, bool IS_B, int ROWS, int THREADS>
@@ -124,9 +146,9 @@ struct Tile {
     static constexpr int CE = Chunk<T>::n;
     static constexpr int BK = ROW_BYTES / (int)sizeof(T);
     static constexpr bool ACROSS = MODE == DW || (MODE == DX && IS_B);
-    static constexpr int CHUNKS = ROWS * 8;
+    static constexpr int CHUNKS = ROWS * (ROW_BYTES / 16);
     static constexpr int PER = CHUNKS / THREADS;
-    static constexpr int CPR = ACROSS ? ROWS / CE : 8;         // chunks of a memory row
+    static constexpr int CPR = ACROSS ? ROWS / CE : ROW_BYTES / 16;         // chunks of a memory row
     static_assert(CHUNKS % THREADS == 0, "whole chunks per thread");
 
     // chunk q of the tile: (row of memory, first element in it, both inside the tile)
@@ -135,29 +157,22 @@ struct Tile {
         const int pos = q % CPR;
         e = (ACROSS ? tile_k_across<T>(r, pos) : tile_k_along(r, pos)) * CE;
     }
-    // address of memory row `r` of the tile that starts at (row0, k0); FWD's B: groups of 32 rows, gate and up in turn
-    static __device__ __forceinline__ const T* row_ptr(const ProductArgs& a, int64_t row0, int64_t k0, int r, int64_t& row, int64_t rows) {
+    // address of memory row `r` of the tile that starts at (row0, k0); FWD's B: groups of 32 rows, gate and up in turn.
+    // Rows of m or n beyond the edge repeat the last one (their results are never stored).
+    static __device__ __forceinline__ const T* row_ptr(const ProductArgs& a, int64_t row0, int64_t rows, int64_t k0, int r, bool second) {
         const Operand& o = IS_B ? a.B : a.A;
         if constexpr (ACROSS) {
-            row = k0 + r;
-            if constexpr (MODE == DX) {
-                const bool second = row >= a.h;
-                return (const T*)(second ? o.p1 : o.p0) + (second ? row - a.h : row) * (second ? o.ld1 : o.ld0);
-            }
-            return (const T*)o.p0 + row * o.ld0;
+            if (MODE == DX && second) return (const T*)o.p1 + (k0 + r) * o.ld1;
+            return (const T*)o.p0 + (k0 + r) * o.ld0;
         } else if constexpr (MODE == FWD && IS_B) {
-            row = row0 / 2 + (r / 64) * 32 + (r & 31);
-            const bool up = (r & 32) != 0;
-            const int64_t rr = row < rows ? row : rows - 1;
-            return (const T*)(up ? o.p1 : o.p0) + rr * (up ? o.ld1 : o.ld0);
+            const int64_t row = row0 / 2 + (r / 64) * 32 + (r & 31), rr = row < rows ? row : rows - 1;
+            return (r & 32) ? (const T*)o.p1 + rr * o.ld1 : (const T*)o.p0 + rr * o.ld0;
         } else {
-            row = row0 + r;
-            const int64_t rr = row < rows ? row : rows - 1;
-            return (const T*)o.p0 + rr * o.ld0;
+            const int64_t row = row0 + r, rr = row < rows ? row : rows - 1;
+            return (const T*)o.p0 + rr * o.ld0 + (MODE == DX && second ? a.half : 0);
         }
     }
-    // The thread's chunks at k = 0, found once: a step then adds one offset to all of them.  DX's B reads the second
-    // weight from k = h on: its chunks at k = h.
+    // The thread's chunks at k = 0, found once: a stage then adds one offset to all of them.  DX's B: of both weights.
     struct Pointers {
         const T* at[PER];
         const T* at2[MODE == DX && IS_B ? PER : 1];
@@ -167,51 +182,37 @@ struct Tile {
         for (int i = 0; i < PER; ++i) {
             int r, e;
             place(i * THREADS + (int)threadIdx.x, r, e);
-            if constexpr (ACROSS) {       // columns beyond the edge repeat the last chunk (their results are never stored)
-                const int64_t col = row0 + e < rows ? row0 + e : rows - CE;
-                const Operand& o = IS_B ? a.B : a.A;
-                p.at[i] = (const T*)o.p0 + r * o.ld0 + col;
-                if constexpr (MODE == DX) p.at2[i] = (const T*)o.p1 + r * o.ld1 + col;
-            } else {                      // rows beyond the edge repeat the last one
-                int64_t row;
-                p.at[i] = row_ptr(a, row0, 0, r, row, rows) + e;
-            }
+            // columns beyond the edge repeat the last chunk
+            const int64_t col = !ACROSS ? e : row0 + e < rows ? row0 + e : (rows - 1) / CE * CE;
+            p.at[i] = row_ptr(a, row0, rows, 0, r, false) + col;
+            if constexpr (MODE == DX && IS_B) p.at2[i] = row_ptr(a, row0, rows, 0, r, true) + col;
         }
     }
-    // direct global -> LDS: every k of the step exists (DX: on one side of h), chunks are aligned and whole
-    static __device__ __forceinline__ void load_direct(const ProductArgs& a, const Pointers& p, int64_t k0, char* lds) {
+    static __device__ __forceinline__ int64_t offset(const ProductArgs& a, int64_t k0, bool second) {
         const Operand& o = IS_B ? a.B : a.A;
-        const bool second = MODE == DX && IS_B && k0 >= a.h;
-        const int64_t step = !ACROSS ? k0 : second ? (k0 - a.h) * o.ld1 : k0 * o.ld0;
+        if constexpr (ACROSS) return k0 * (MODE == DX && second ? o.ld1 : o.ld0);
+        return k0 + (MODE == DX && second ? a.half : 0);
+    }
+    // whole stage from k0 on, direct global -> LDS
+    static __device__ __forceinline__ void load_direct(const ProductArgs& a, const Pointers& p, int64_t k0, bool second, char* lds) {
+        const int64_t step = offset(a, k0, second);
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const T* src = p.at[i];
             if constexpr (MODE == DX && IS_B) src = second ? p.at2[i] : src;
-            char* dst = lds + (size_t)(i * THREADS + (threadIdx.x & ~63)) * 16;
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + step),
-                                             (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+            load_to_lds(src + step, lds + (i * THREADS + (threadIdx.x & ~63)) * 16);
         }
     }
-    // through registers: any alignment, zeros beyond the edges
-    static __device__ __forceinline__ void load_masked(const ProductArgs& a, int64_t row0, int64_t rows, int64_t k0, int64_t k_end, Vec<T> (&v)[PER]) {
+    // ragged stage, through registers: zeros from k = K on and beyond the edges of across tiles
+    static __device__ __forceinline__ void load_masked(const ProductArgs& a, int64_t row0, int64_t rows, int64_t k0, bool second, char* lds) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             int r, e;
             place(i * THREADS + (int)threadIdx.x, r, e);
-            int64_t row, left;
-            if constexpr (ACROSS) {
-                left = k0 + r < k_end ? rows - (row0 + e) : 0;
-                const T* p = row_ptr(a, row0, left > 0 ? k0 : 0, left > 0 ? r : 0, row, rows) + row0 + e;
-                v[i] = load_part(p, left);
-            } else {
-                left = k_end - (k0 + e);
-                v[i] = load_part(row_ptr(a, row0, k0, r, row, rows) + k0 + e, left);
-            }
+            const int64_t left = !ACROSS ? a.K - (k0 + e) : k0 + r < a.K ? rows - (row0 + e) : 0;
+            const T* p = row_ptr(a, row0, rows, left > 0 ? k0 : 0, left > 0 ? r : 0, second) + (ACROSS ? row0 + e : k0 + e);
+            *(Vec<T>*)(lds + (size_t)(i * THREADS + threadIdx.x) * 16) = load_part(p, left);
         }
-    }
-    static __device__ __forceinline__ void store_lds(char* lds, const Vec<T> (&v)[PER]) {
-#pragma unroll
-        for (int i = 0; i < PER; ++i) *(Vec<T>*)(lds + (size_t)(i * THREADS + threadIdx.x) * 16) = v[i];
     }
     // the lane's operand of the 32 rows from `base` on for k step ks (16 elements of k, float32: 8)
     static __device__ __forceinline__ typename Frag<T>::type frag(const char* lds, int base, int ks, int lane) {
@@ -259,120 +260,170 @@ __device__ __forceinline__ void tile_of(int id, int tiles_m, int tiles_n, int& t
     tn = in / height;
 }
 
-template <typename T, int MODE, int BM, int BN, int WM, int WN, bool DIRECT>
+// until at most AHEAD - 1 stages (fewer asked for: none), of LOADS loads a thread, are under way
+template <int LOADS> __device__ __forceinline__ void wait_loads(int stages) {
+    if (stages >= AHEAD - 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((AHEAD - 1) * LOADS) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+// every wave's LDS accesses so far are done, and no wave goes on before that
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+template <typename T, int MODE, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs args) {
     constexpr int THREADS = WM * WN * 64;
     using TA = Tile<T, MODE, false, BM, THREADS>;
     using TB = Tile<T, MODE, true, BN, THREADS>;
-    constexpr int BK = TA::BK, KSTEPS = BK / (sizeof(T) == 2 ? 16 : 8);
+    constexpr int BK = TA::BK;
     constexpr int MI = BM / WM / 32, NI = BN / WN / 32;
-    constexpr int A_BYTES = BM * ROW_BYTES, B_BYTES = BN * ROW_BYTES, BUF = A_BYTES + B_BYTES;
-    static_assert(MODE != FWD || NI == 2, "one gate and one up group per wave");
+    constexpr int A_BYTES = BM * ROW_BYTES, BUF = A_BYTES + BN * ROW_BYTES;
+    constexpr int LOADS = TA::PER + TB::PER;
+    static_assert(MODE != FWD || NI % 2 == 0, "gate and up groups in pairs");
+    static_assert(BK / (sizeof(T) == 2 ? 16 : 8) == 2, "two k steps a stage");
     extern __shared__ __align__(128) char lds[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
     int tm, tn;
     tile_of(blockIdx.x, args.tiles_m, args.tiles_n, tm, tn);
     const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;              // FWD: n0 counts gate and up rows
-    const int64_t k_begin = (int64_t)blockIdx.y * args.k_chunk;
-    const int64_t k_end = k_begin + args.k_chunk < args.K ? k_begin + args.k_chunk : args.K;
-    const int steps = (int)((k_end - k_begin + BK - 1) / BK);
+    // Stages of k: the ragged ends first (DX: of da and of db), then the whole ones, so that all but the first few go the
+    // direct way.  This block's slice of them: [first, last).
+    const int whole = (int)(args.K / BK), ragged = args.K % BK ? (MODE == DX ? 2 : 1) : 0, all = ragged + whole * (MODE == DX ? 2 : 1);
+    const int first = blockIdx.y * args.stages, last = first + args.stages < all ? first + args.stages : all;
     floatx16 acc[MI][NI] = {};
-    Vec<T> va[TA::PER], vb[TB::PER];
     typename TA::Pointers pa;
     typename TB::Pointers pb;
-    if (DIRECT) { TA::pointers(args, m0, args.M, pa); TB::pointers(args, n0, args.N, pb); }
+    TA::pointers(args, m0, args.M, pa);
+    TB::pointers(args, n0, args.N, pb);
 
-    // Step s into `buf`: direct loads, or (a ragged step; every step if !DIRECT) into registers, which commit() stores.
-    auto fetch = [&](int s, char* buf) {
-        const int64_t k0 = k_begin + (int64_t)s * BK;
-        if (DIRECT && k0 + BK <= k_end && (MODE != DX || k0 + BK <= args.h || k0 >= args.h)) {
-            TA::load_direct(args, pa, k0, buf);
-            TB::load_direct(args, pb, k0, buf + A_BYTES);
-        } else {
-            TA::load_masked(args, m0, args.M, k0, k_end, va);
-            TB::load_masked(args, n0, args.N, k0, k_end, vb);
-            if (DIRECT) { TA::store_lds(buf, va); TB::store_lds(buf + A_BYTES, vb); }
-        }
-    };
-    auto commit = [&](char* buf) {
-        if (!DIRECT) { TA::store_lds(buf, va); TB::store_lds(buf + A_BYTES, vb); }
+    auto load_whole = [&](int s, char* buf) {
+        const int q = s - ragged;
+        const bool second = MODE == DX && q >= whole;
+        const int64_t k0 = (int64_t)(second ? q - whole : q) * BK;
+        TA::load_direct(args, pa, k0, second, buf);
+        TB::load_direct(args, pb, k0, second, buf + A_BYTES);
     };
     typename Frag<T>::type fa[2][MI], fb[2][NI];
-    auto read = [&](const char* buf, int ks, int to) {
+    auto read = [&](const char* buf, int ks) {
 #pragma unroll
-        for (int i = 0; i < MI; ++i) fa[to][i] = TA::frag(buf, wm * (BM / WM) + 32 * i, ks, lane);
+        for (int i = 0; i < MI; ++i) fa[ks][i] = TA::frag(buf, wm * (BM / WM) + 32 * i, ks, lane);
 #pragma unroll
-        for (int j = 0; j < NI; ++j) fb[to][j] = TB::frag(buf + A_BYTES, wn * (BN / WN) + 32 * j, ks, lane);
+        for (int j = 0; j < NI; ++j) fb[ks][j] = TB::frag(buf + A_BYTES, wn * (BN / WN) + 32 * j, ks, lane);
     };
-    auto multiply = [&](int from) {
+    auto multiply = [&](int ks, int from, int to) {
 #pragma unroll
-        for (int i = 0; i < MI; ++i)
+        for (int i = from; i < to; ++i)
 #pragma unroll
-            for (int j = 0; j < NI; ++j) acc[i][j] = mma(T(), fa[from][i], fb[from][j], acc[i][j]);
+            for (int j = 0; j < NI; ++j) acc[i][j] = mma(T(), fa[ks][i], fb[ks][j], acc[i][j]);
     };
-    // Operands are read one k step ahead of their use, and the barrier between two buffers stands before the last
-    // k step's products, which cover the first reads of the new buffer.
-    fetch(0, lds);
-    commit(lds);
-    __syncthreads();
-    read(lds, 0, 0);
-    for (int s = 0; s < steps; ++s) {
-        char* cur = lds + (s & 1) * BUF;
-        char* nxt = lds + ((s + 1) & 1) * BUF;
-        if (s + 1 < steps) fetch(s + 1, nxt);
+    // order of a half stage's instructions: a product first (its operands are there), then the reads among the others
+    auto interleave = [&](auto rows) {
+        constexpr int across = sizeof(T) == 2 ? 2 : 4;
+        constexpr int READS = MI * (TA::ACROSS ? across : 1) + NI * (TB::ACROSS ? across : 1);
+        constexpr int PRODUCTS = decltype(rows)::value * NI * (sizeof(T) == 4 ? 4 : 1), EACH = (READS + PRODUCTS - 2) / (PRODUCTS - 1);
 #pragma unroll
-        for (int ks = 0; ks + 1 < KSTEPS; ++ks) {
-            read(cur, ks + 1, (ks + 1) & 1);
-            multiply(ks & 1);
+        for (int i = 0; i < PRODUCTS; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, EACH, 0);
         }
-        if (s + 1 < steps) commit(nxt);
-        __syncthreads();
-        if (s + 1 < steps) read(nxt, 0, 0);
-        multiply((KSTEPS - 1) & 1);
+    };
+    for (int t = 0; t < AHEAD && first + t < last; ++t) {
+        const int s = first + t;
+        char* buf = lds + t * BUF;
+        if (s >= ragged) load_whole(s, buf);
+        else {                                    // its loads are waited for at once, and with them all earlier ones
+            TA::load_masked(args, m0, args.M, (int64_t)whole * BK, s == 1, buf);
+            TB::load_masked(args, n0, args.N, (int64_t)whole * BK, s == 1, buf + A_BYTES);
+        }
     }
-    // register v of a lane: row 8 (v / 4) + 4 (lane / 32) + v % 4, column lane % 32
-    const int hl = lane >> 5, col = lane & 31;
-    if constexpr (MODE == FWD) {
-        const int64_t n = n0 / 2 + wn * 32 + col;
-        if (n >= args.N) return;
-        by_act(args.act, [&](auto kind) {
-            constexpr int ACT = decltype(kind)::value;
+    wait_loads<LOADS>(last - first - 1);
+    lds_barrier();
+    read(lds, 0);
+    // One stage a turn: the products of its first half, among them the loads of the stage three ahead and the reads of its
+    // second half; the barrier; the products of the second half, which cover the first reads of the next stage.  A stage is
+    // loaded into the place of the one two before: what any wave read there it had used before the last barrier.  (The last
+    // turns load nothing, and the very last reads a half stage that it does not use.)
+    int cur = 0, fill = AHEAD * BUF;
+    for (int s = first; s < last; ++s) {
+        const bool more = s + AHEAD < last;
+        multiply(0, 0, 1);
+        if (more) load_whole(s + AHEAD, lds + fill);
+        read(lds + cur, 1);
+        multiply(0, 1, MI);
+        interleave(std::integral_constant<int, MI - 1>{});
+        fill = fill == (STAGES - 1) * BUF ? 0 : fill + BUF;
+        cur = cur == (STAGES - 1) * BUF ? 0 : cur + BUF;
+        wait_loads<LOADS>(more ? AHEAD - 1 : 0);
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        read(lds + cur, 0);
+        multiply(1, 0, MI);
+        interleave(std::integral_constant<int, MI>{});
+    }
+    // Results through LDS, 32 rows of the wave at a time in a corner of its own: register v of a lane is row
+    // 8 (v / 4) + 4 (lane / 32) + v % 4, column lane % 32; what leaves are 16-byte chunks of whole rows.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    lds_barrier();
+    constexpr int COLS = NI * 32, PITCH = COLS + 4;               // floats; the pitch spreads the rows over the banks
+    static_assert(WM * WN * 32 * PITCH * 4 <= STAGES * BUF, "the corners fit");
+    float* corner = (float*)lds + wave * (32 * PITCH);
 #pragma unroll
-            for (int i = 0; i < MI; ++i)
+    for (int i = 0; i < MI; ++i) {
 #pragma unroll
-                for (int v = 0; v < 16; ++v) {
-                    const int64_t m = m0 + wm * (BM / WM) + 32 * i + 8 * (v / 4) + 4 * hl + v % 4;
-                    if (m >= args.M) continue;
-                    gate_out<T, ACT>(args, m * args.N + n, acc[i][0][v], acc[i][1][v]);
+        for (int j = 0; j < NI; ++j)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) corner[(8 * (v / 4) + 4 * (lane >> 5) + v % 4) * PITCH + 32 * j + (lane & 31)] = acc[i][j][v];
+        const int64_t row0 = m0 + wm * (BM / WM) + 32 * i;
+        if constexpr (MODE == FWD) {
+            constexpr int CE = Chunk<T>::n, PER_ROW = COLS / 2 / CE;
+            by_act(args.act, [&](auto kind) {
+                constexpr int ACT = decltype(kind)::value;
+#pragma unroll 2
+                for (int q = lane; q < 32 * PER_ROW; q += 64) {
+                    const int r = q / PER_ROW, c = q % PER_ROW * CE;                  // c: column among the wave's outputs
+                    const float* g = corner + r * PITCH + c / 32 * 64 + c % 32;
+                    const int64_t m = row0 + r, n = n0 / 2 + wn * (COLS / 2) + c, left = m < args.M ? args.N - n : 0;
+                    if (left > 0) gate_out<T, ACT>(args, m * args.N + n, g, g + 32, left);
                 }
-        });
-    } else {
+            });
+        } else if (args.partial) {
+            constexpr int PER_ROW = COLS / 4;
+            for (int q = lane; q < 32 * PER_ROW; q += 64) {
+                const int r = q / PER_ROW, c = q % PER_ROW * 4;
+                const int64_t m = row0 + r, n = n0 + wn * COLS + c, left = m < args.M ? args.N - n : 0;
+                if (left > 0) store_part(args.partial + ((int64_t)blockIdx.y * args.M + m) * args.N + n, *(const Vec<float>*)(corner + r * PITCH + c), left);
+            }
+        } else {
+            constexpr int CE = Chunk<T>::n, PER_ROW = COLS / CE;
+#pragma unroll 2
+            for (int q = lane; q < 32 * PER_ROW; q += 64) {
+                const int r = q / PER_ROW, c = q % PER_ROW * CE;
+                const int64_t n = n0 + wn * COLS + c;
+                int64_t m = row0 + r;
+                T* out = (T*)args.out0;
+                if (MODE == DW && m >= args.half) { m -= args.half; out = (T*)args.out1; }
+                const int64_t left = m < (MODE == DW ? args.h : args.M) ? args.N - n : 0;
+                if (left <= 0) continue;
+                Vec<T> o;
 #pragma unroll
-        for (int j = 0; j < NI; ++j) {
-            const int64_t n = n0 + wn * (BN / WN) + 32 * j + col;
-            if (n >= args.N) continue;
-#pragma unroll
-            for (int i = 0; i < MI; ++i)
-#pragma unroll
-                for (int v = 0; v < 16; ++v) {
-                    const int64_t m = m0 + wm * (BM / WM) + 32 * i + 8 * (v / 4) + 4 * hl + v % 4;
-                    if (m >= args.M) continue;
-                    if (args.partial) args.partial[((int64_t)blockIdx.y * args.M + m) * args.N + n] = acc[i][j][v];
-                    else if (MODE == DW && m >= args.h) ((T*)args.out1)[(m - args.h) * args.N + n] = from_f32<T>(acc[i][j][v]);
-                    else ((T*)args.out0)[m * args.N + n] = from_f32<T>(acc[i][j][v]);
-                }
+                for (int e = 0; e < CE; ++e) o.e[e] = from_f32<T>(corner[r * PITCH + c + e]);
+                store_part(out + m * args.N + n, o, left);
+            }
         }
     }
 }
 
-// Sum of the k slices, rounded once.  `first` elements go to out0, the rest to out1.
+// Sum of the k slices [slices][2][at1 or n], rounded once: elements [0, n0) to out0, [at1, at1 + n0) to out1
 template <typename T>
-__global__ __launch_bounds__(256) void sum_slices_kernel(const float* __restrict__ partial, int slices, int64_t n, int64_t first, T* __restrict__ out0, T* __restrict__ out1) {
+__global__ __launch_bounds__(256) void sum_slices_kernel(const float* __restrict__ partial, int slices, int64_t n, int64_t n0, int64_t at1, T* __restrict__ out0, T* __restrict__ out1) {
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        if (i >= n0 && (i < at1 || i >= at1 + n0)) continue;
         float s = 0.0f;
         for (int z = 0; z < slices; ++z) s += partial[z * n + i];
-        if (i < first) out0[i] = from_f32<T>(s);
-        else out1[i - first] = from_f32<T>(s);
+        if (i < n0) out0[i] = from_f32<T>(s);
+        else out1[i - at1] = from_f32<T>(s);
     }
 }
 
@@ -433,28 +484,31 @@ __global__ __launch_bounds__(512) void gated_few_rows_kernel(const ProductArgs a
 #pragma unroll
             for (int v = 0; v < 16; ++v) part[(((wave * MT + i) * 2 + w) * 16 + v) * 64 + lane] = acc[i][w][v];
     __syncthreads();
-    if (j >= args.N) return;
     by_act(args.act, [&](auto kind) {
         constexpr int ACT = decltype(kind)::value;
-        for (int iv = wave; iv < 16 * MT; iv += WAVES) {
-            const int i = iv / 16, v = iv % 16;
-            const int64_t t = 32 * i + 8 * (v / 4) + 4 * hl + v % 4;
-            if (t >= args.M) continue;
-            float a = 0.0f, b = 0.0f;
+        const int64_t j0 = (int64_t)blockIdx.x * 32;
+        for (int q = threadIdx.x; q < MT * 32 * (32 / CE); q += 512) {
+            const int t = q / (32 / CE), c = q % (32 / CE) * CE;
+            if (t >= args.M || j0 + c >= args.N) continue;
+            // row t is register v of half wave `half` in row tile t / 32
+            const int tt = t % 32, v = 4 * (tt / 8) + tt % 4, half = (tt / 4) % 2;
+            float a[CE] = {}, b[CE] = {};
 #pragma unroll
-            for (int w = 0; w < WAVES; ++w) {
-                a += part[(((w * MT + i) * 2 + 0) * 16 + v) * 64 + lane];
-                b += part[(((w * MT + i) * 2 + 1) * 16 + v) * 64 + lane];
-            }
-            gate_out<T, ACT>(args, t * args.N + j, a, b);
+            for (int w = 0; w < WAVES; ++w)
+#pragma unroll
+                for (int e = 0; e < CE; ++e) {
+                    a[e] += part[(((w * MT + t / 32) * 2 + 0) * 16 + v) * 64 + 32 * half + c + e];
+                    b[e] += part[(((w * MT + t / 32) * 2 + 1) * 16 + v) * 64 + 32 * half + c + e];
+                }
+            gate_out<T, ACT>(args, t * args.N + j0 + c, a, b, args.N - (j0 + c));
         }
     });
 }
 
-// [da | db] = [gy p | gy f] of every row: bandwidth (three reads, two writes of T h)
+// da = gy p and, `half` columns behind it, db = gy f of every row: bandwidth (three reads, two writes of T h)
 template <typename T>
 __global__ __launch_bounds__(256) void gated_da_db_kernel(const T* __restrict__ f, const T* __restrict__ p, const T* __restrict__ gy, int64_t ldgy,
-                                                           T* __restrict__ dab, int64_t rows, int64_t h) {
+                                                           T* __restrict__ dab, int64_t half, int64_t rows, int64_t h) {
     constexpr int CE = Chunk<T>::n;
     const int64_t per = (h + CE - 1) / CE;
     for (int64_t t = blockIdx.y; t < rows; t += gridDim.y)
@@ -468,47 +522,40 @@ __global__ __launch_bounds__(256) void gated_da_db_kernel(const T* __restrict__ 
                 da.e[i] = from_f32<T>(g * to_f32(vp.e[i]));
                 db.e[i] = from_f32<T>(g * to_f32(vf.e[i]));
             }
-            store_part(dab + t * 2 * h + c, da, left);
-            store_part(dab + t * 2 * h + h + c, db, left);
+            store_part(dab + t * 2 * half + c, da, left);
+            store_part(dab + t * 2 * half + half + c, db, left);
         }
 }
 
 // -- host ------------------------------------------------------------------------------------------------------------
-template <typename T> bool whole(const void* p, int64_t ld, int64_t n) {
-    return ((uintptr_t)p & 15) == 0 && ld % Chunk<T>::n == 0 && n % Chunk<T>::n == 0;
-}
-
-struct Plan { bool big; int slices; int64_t k_chunk; };
+struct Plan { bool big; int slices, stages; };
 
 // Tile and split of one product.  256 x 256 tiles (one block of eight waves per CU) where they fill the chip, else
-// 128 x 128 (two blocks per CU); if those do not fill it either, the k range is cut into slices of at least eight steps.
+// 128 x 128 (two blocks per CU); if those do not fill it either, k is cut into slices of at least sixteen stages.
 template <typename T> Plan plan_of(int mode, int64_t M, int64_t N, int64_t K) {
     const int cus = marl_net::device_cus(256);
-    const int64_t bk = ROW_BYTES / sizeof(T);
-    Plan p;
+    const int64_t bk = ROW_BYTES / sizeof(T), all = (K + bk - 1) / bk * (mode == DX ? 2 : 1);
     auto tiles = [&](int64_t b) { return ((M + b - 1) / b) * ((N + b - 1) / b); };
-    const int64_t steps = K > 0 ? (K + bk - 1) / bk : 1;
-    p.big = tiles(256) >= cus * 3 / 4;
-    p.slices = 1;
+    Plan p = {tiles(256) >= cus * 3 / 4, 1, (int)all};
     if (mode != FWD && !p.big) {
-        const int64_t want = 2 * cus / tiles(128);
-        p.slices = (int)(want < 1 ? 1 : want < steps / 8 ? want : steps / 8 < 1 ? 1 : steps / 8);
+        const int64_t want = 2 * cus / tiles(128), most = all / 16;
+        const int64_t slices = want < 1 ? 1 : want < most ? want : most < 1 ? 1 : most;
+        p.stages = (int)((all + slices - 1) / slices);
+        p.slices = (int)((all + p.stages - 1) / p.stages);
     }
-    p.k_chunk = ((steps + p.slices - 1) / p.slices) * bk;
-    p.slices = (int)((steps * bk + p.k_chunk - 1) / p.k_chunk);
     return p;
 }
 
-template <typename T, int MODE, int BM, int WM, int WN, bool DIRECT>
+template <typename T, int MODE, int BM, int WM, int WN>
 hipError_t launch_tiles(ProductArgs& a, int64_t n_virtual, const Plan& p, hipStream_t stream) {
     static bool attr_set[marl_net::kMaxDevices];
-    auto* kernel = product_kernel<T, MODE, BM, BM, WM, WN, DIRECT>;
-    const size_t bytes = (size_t)4 * BM * ROW_BYTES;
+    auto* kernel = product_kernel<T, MODE, BM, BM, WM, WN>;
+    const size_t bytes = (size_t)STAGES * 2 * BM * ROW_BYTES;
     hipError_t err = marl_net::allow_dynamic_lds((const void*)kernel, bytes, attr_set);
     if (err != hipSuccess) return err;
     a.tiles_m = (int)((a.M + BM - 1) / BM);
     a.tiles_n = (int)((n_virtual + BM - 1) / BM);
-    a.k_chunk = p.k_chunk;
+    a.stages = p.stages;
     hipLaunchKernelGGL(kernel, dim3(a.tiles_m * a.tiles_n, p.slices), dim3(WM * WN * 64), bytes, stream, a);
     return hipGetLastError();
 }
@@ -518,18 +565,12 @@ hipError_t launch_product(ProductArgs& a, float* partial, hipStream_t stream) {
     const int64_t n_virtual = MODE == FWD ? ((a.N + 31) / 32) * 64 : a.N;       // FWD: gate and up in groups of 32
     const Plan p = plan_of<T>(MODE, a.M, n_virtual, a.K);
     a.partial = p.slices > 1 ? partial : nullptr;
-    // direct loads: whole aligned chunks in both operands.  k along the row: the ragged end goes through registers
-    bool direct = MODE == DW ? whole<T>(a.A.p0, a.A.ld0, a.M) && whole<T>(a.B.p0, a.B.ld0, a.N)
-                             : whole<T>(a.A.p0, a.A.ld0, 0) && whole<T>(a.B.p0, a.B.ld0, MODE == DX ? a.N : 0) &&
-                                   whole<T>(a.B.p1, a.B.ld1, MODE == DX ? a.N : 0);
-    hipError_t err;
-    if (p.big) err = direct ? launch_tiles<T, MODE, 256, 2, 4, true>(a, n_virtual, p, stream) : launch_tiles<T, MODE, 256, 2, 4, false>(a, n_virtual, p, stream);
-    else err = direct ? launch_tiles<T, MODE, 128, 2, 2, true>(a, n_virtual, p, stream) : launch_tiles<T, MODE, 128, 2, 2, false>(a, n_virtual, p, stream);
+    const hipError_t err = p.big ? launch_tiles<T, MODE, 256, 2, 4>(a, n_virtual, p, stream) : launch_tiles<T, MODE, 128, 2, 2>(a, n_virtual, p, stream);
     if (err != hipSuccess || a.partial == nullptr) return err;
     const int64_t n = a.M * a.N;
-    const int64_t first = MODE == DW ? a.h * a.N : n;
     const int64_t blocks = (n + 255) / 256;
-    hipLaunchKernelGGL(sum_slices_kernel<T>, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, stream, partial, p.slices, n, first, (T*)a.out0, (T*)a.out1);
+    hipLaunchKernelGGL(sum_slices_kernel<T>, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, stream, partial, p.slices, n,
+                       MODE == DW ? a.h * a.N : n, MODE == DW ? a.half * a.N : n, (T*)a.out0, (T*)a.out1);
     return hipGetLastError();
 }
 
@@ -542,48 +583,86 @@ template <typename T, int MT> hipError_t launch_few_rows(const ProductArgs& a, h
     return hipGetLastError();
 }
 
-template <typename T> int forward(int act, int64_t rows, int32_t d, int32_t h, const void* x, int64_t ldx, const void* wg, int64_t ldg,
-                                  const void* wu, int64_t ldu, void* y, void* f, void* p, hipStream_t stream) {
+int64_t round_256(int64_t n) { return (n + 255) / 256 * 256; }
+
+// Rows of `n` elements as the product kernel takes them: 16-byte aligned, whole chunks readable (what is behind a row's
+// end inside its last chunk meets only zeros or results that are not stored).
+struct Matrix { const void* p; int64_t ld, rows; };
+template <typename T> bool aligned(const Matrix& m, int64_t n) { return ((uintptr_t)m.p & 15) == 0 && m.ld % Chunk<T>::n == 0 && n % Chunk<T>::n == 0; }
+template <typename T> int64_t packed_ld(int64_t n) { return (n + Chunk<T>::n - 1) / Chunk<T>::n * Chunk<T>::n; }
+template <typename T> size_t packed_bytes(const Matrix& m, int64_t n) {
+    return aligned<T>(m, n) ? 0 : (size_t)round_256(m.rows * packed_ld<T>(n) * (int64_t)sizeof(T));
+}
+template <typename T>
+__global__ __launch_bounds__(256) void pack_rows_kernel(const T* __restrict__ src, int64_t ld, T* __restrict__ dst, int64_t rows, int64_t n, int64_t per) {
+    constexpr int CE = Chunk<T>::n;
+    for (int64_t r = blockIdx.y; r < rows; r += gridDim.y)
+        for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < per; q += (int64_t)gridDim.x * 256)
+            *(Vec<T>*)(dst + (r * per + q) * CE) = load_part(src + r * ld + q * CE, n - q * CE);
+}
+// m itself, or its copy in the workspace (which moves on)
+template <typename T> Matrix pack(const Matrix& m, int64_t n, char*& ws, hipStream_t stream) {
+    const size_t bytes = packed_bytes<T>(m, n);
+    if (bytes == 0) return m;
+    const Matrix to = {ws, packed_ld<T>(n), m.rows};
+    ws += bytes;
+    const int64_t per = to.ld / Chunk<T>::n;
+    hipLaunchKernelGGL(pack_rows_kernel<T>, dim3((unsigned)((per + 255) / 256), (unsigned)(m.rows < 65535 ? m.rows : 65535)), dim3(256), 0, stream,
+                       (const T*)m.p, m.ld, (T*)to.p, m.rows, n, per);
+    return to;
+}
+
+struct Gated { int64_t rows; int32_t d, h; Matrix x, wg, wu; };
+constexpr int FEW_ROWS = 64;              // up to here the forward product reads its operands as they are
+
+template <typename T> size_t workspace(const Gated& g, bool backward) {
+    const size_t packed = backward || g.rows > FEW_ROWS ? packed_bytes<T>(g.x, g.d) + packed_bytes<T>(g.wg, g.d) + packed_bytes<T>(g.wu, g.d) : 0;
+    if (!backward) return packed;
+    const int64_t h2 = 2 * packed_ld<T>(g.h);
+    const Plan px = plan_of<T>(DX, g.rows, g.d, g.h), pw = plan_of<T>(DW, h2, g.d, g.rows);
+    const int64_t sx = px.slices > 1 ? px.slices * g.rows * g.d : 0, sw = pw.slices > 1 ? pw.slices * h2 * g.d : 0;
+    return packed + (size_t)(round_256(g.rows * h2 * (int64_t)sizeof(T)) + (sx > sw ? sx : sw) * (int64_t)sizeof(float));
+}
+
+template <typename T> int forward(int act, Gated g, void* y, void* f, void* p, void* workspace, hipStream_t stream) {
     ProductArgs a = {};
-    a.A = {x, nullptr, ldx, 0};
-    a.B = {wg, wu, ldg, ldu};
-    a.M = rows; a.N = h; a.K = d; a.h = h;
+    char* ws = (char*)workspace;
+    if (g.rows > FEW_ROWS) { g.x = pack<T>(g.x, g.d, ws, stream); g.wg = pack<T>(g.wg, g.d, ws, stream); g.wu = pack<T>(g.wu, g.d, ws, stream); }
+    a.A = {g.x.p, nullptr, g.x.ld, 0};
+    a.B = {g.wg.p, g.wu.p, g.wg.ld, g.wu.ld};
+    a.M = g.rows; a.N = g.h; a.K = g.d; a.h = g.h;
     a.out0 = y; a.save_f = f; a.save_p = p; a.act = act;
-    hipError_t err = rows <= 32 ? launch_few_rows<T, 1>(a, stream) : rows <= 64 ? launch_few_rows<T, 2>(a, stream) : launch_product<T, FWD>(a, nullptr, stream);
+    const hipError_t err = g.rows <= 32 ? launch_few_rows<T, 1>(a, stream) : g.rows <= FEW_ROWS ? launch_few_rows<T, 2>(a, stream)
+                                                                                                : launch_product<T, FWD>(a, nullptr, stream);
     if (err == hipSuccess) return MARL_OK;
     marl_note_hip_error((int)err);
     return MARL_EHIP;
 }
 
-int64_t round_256(int64_t n) { return (n + 255) / 256 * 256; }
-
-template <typename T> size_t workspace(int64_t rows, int32_t d, int32_t h) {
-    const Plan px = plan_of<T>(DX, rows, d, 2 * (int64_t)h), pw = plan_of<T>(DW, 2 * (int64_t)h, d, rows);
-    const int64_t sx = px.slices > 1 ? px.slices * rows * d : 0, sw = pw.slices > 1 ? pw.slices * 2 * (int64_t)h * d : 0;
-    return (size_t)(round_256(rows * 2 * h * (int64_t)sizeof(T)) + (sx > sw ? sx : sw) * (int64_t)sizeof(float));
-}
-
-template <typename T> int backward(int64_t rows, int32_t d, int32_t h, const void* x, int64_t ldx, const void* wg, int64_t ldg,
-                                   const void* wu, int64_t ldu, const void* f, const void* p, const void* gy, int64_t ldgy, void* dx,
-                                   void* dwg, void* dwu, void* ws, hipStream_t stream) {
+template <typename T> int backward(Gated g, const void* f, const void* p, const void* gy, int64_t ldgy, void* dx, void* dwg, void* dwu,
+                                   void* workspace, hipStream_t stream) {
+    char* ws = (char*)workspace;
+    const int64_t half = packed_ld<T>(g.h), per = half / Chunk<T>::n;
     T* dab = (T*)ws;
-    float* partial = (float*)((char*)ws + round_256(rows * 2 * h * (int64_t)sizeof(T)));
-    const int64_t per = (h + Chunk<T>::n - 1) / Chunk<T>::n;
-    hipLaunchKernelGGL(gated_da_db_kernel<T>, dim3((unsigned)((per + 255) / 256), (unsigned)(rows < 65535 ? rows : 65535)), dim3(256), 0, stream,
-                       (const T*)f, (const T*)p, (const T*)gy, ldgy, dab, rows, (int64_t)h);
+    ws += round_256(g.rows * 2 * half * (int64_t)sizeof(T));
+    hipLaunchKernelGGL(gated_da_db_kernel<T>, dim3((unsigned)((per + 255) / 256), (unsigned)(g.rows < 65535 ? g.rows : 65535)), dim3(256), 0, stream,
+                       (const T*)f, (const T*)p, (const T*)gy, ldgy, dab, half, g.rows, (int64_t)g.h);
     hipError_t err = hipGetLastError();
+    if (err == hipSuccess && dx) { g.wg = pack<T>(g.wg, g.d, ws, stream); g.wu = pack<T>(g.wu, g.d, ws, stream); }
+    if (err == hipSuccess && dwg) g.x = pack<T>(g.x, g.d, ws, stream);
+    float* partial = (float*)ws;
     if (err == hipSuccess && dx) {
         ProductArgs a = {};
-        a.A = {dab, nullptr, 2 * (int64_t)h, 0};
-        a.B = {wg, wu, ldg, ldu};
-        a.M = rows; a.N = d; a.K = 2 * (int64_t)h; a.h = h; a.out0 = dx;
+        a.A = {dab, nullptr, 2 * half, 0};
+        a.B = {g.wg.p, g.wu.p, g.wg.ld, g.wu.ld};
+        a.M = g.rows; a.N = g.d; a.K = g.h; a.h = g.h; a.half = half; a.out0 = dx;
         err = launch_product<T, DX>(a, partial, stream);
     }
     if (err == hipSuccess && dwg) {
         ProductArgs a = {};
-        a.A = {dab, nullptr, 2 * (int64_t)h, 0};
-        a.B = {x, nullptr, ldx, 0};
-        a.M = 2 * (int64_t)h; a.N = d; a.K = rows; a.h = h; a.out0 = dwg; a.out1 = dwu;
+        a.A = {dab, nullptr, 2 * half, 0};
+        a.B = {g.x.p, nullptr, g.x.ld, 0};
+        a.M = 2 * half; a.N = g.d; a.K = g.rows; a.h = g.h; a.half = half; a.out0 = dwg; a.out1 = dwu;
         err = launch_product<T, DW>(a, partial, stream);
     }
     if (err == hipSuccess) return MARL_OK;
@@ -605,18 +684,22 @@ int check_sizes(int32_t dtype, int32_t act, int64_t rows, int32_t d, int32_t h) 
 extern "C" {
 
 int marl_gated_forward(int32_t dtype, int32_t act, int64_t rows, int32_t d, int32_t h, const void* x, int64_t ldx, const void* w_gate,
-                       int64_t ld_gate, const void* w_up, int64_t ld_up, void* y, void* f, void* p, void* stream) {
+                       int64_t ld_gate, const void* w_up, int64_t ld_up, void* y, void* f, void* p, void* workspace_, void* stream) {
     const int rc = check_sizes(dtype, act, rows, d, h);
     if (rc != MARL_OK) return rc;
-    if (!x || !w_gate || !w_up || !y || (f == nullptr) != (p == nullptr)) return MARL_EINVAL;
+    if (!x || !w_gate || !w_up || !y || (f == nullptr) != (p == nullptr) || ((uintptr_t)workspace_ & 15)) return MARL_EINVAL;
     if (ldx < d && rows > 1) return MARL_EINVAL;
     if ((ld_gate < d || ld_up < d) && h > 1) return MARL_EINVAL;
-    return MARL_BY_TYPE(dtype, forward, act, rows, d, h, x, ldx, w_gate, ld_gate, w_up, ld_up, y, f, p, (hipStream_t)stream);
+    const Gated g = {rows, d, h, {x, ldx, rows}, {w_gate, ld_gate, h}, {w_up, ld_up, h}};
+    if (!workspace_ && MARL_BY_TYPE(dtype, workspace, g, false) > 0) return MARL_EINVAL;
+    return MARL_BY_TYPE(dtype, forward, act, g, y, f, p, workspace_, (hipStream_t)stream);
 }
 
-size_t marl_gated_workspace_bytes(int32_t dtype, int64_t rows, int32_t d, int32_t h) {
+size_t marl_gated_workspace_bytes(int32_t dtype, int64_t rows, int32_t d, int32_t h, const void* x, int64_t ldx, const void* w_gate,
+                                  int64_t ld_gate, const void* w_up, int64_t ld_up, int32_t backward_) {
     if (check_sizes(dtype, MARL_ACT_SILU, rows, d, h) != MARL_OK) return 0;
-    return MARL_BY_TYPE(dtype, workspace, rows, d, h);
+    const Gated g = {rows, d, h, {x, ldx, rows}, {w_gate, ld_gate, h}, {w_up, ld_up, h}};
+    return MARL_BY_TYPE(dtype, workspace, g, backward_ != 0);
 }
 
 int marl_gated_backward(int32_t dtype, int64_t rows, int32_t d, int32_t h, const void* x, int64_t ldx, const void* w_gate,
@@ -627,8 +710,8 @@ int marl_gated_backward(int32_t dtype, int64_t rows, int32_t d, int32_t h, const
     if (!x || !w_gate || !w_up || !f || !p || !gy || !workspace_ || ((uintptr_t)workspace_ & 15) || (dw_gate == nullptr) != (dw_up == nullptr)) return MARL_EINVAL;
     if ((ldx < d || ld_gy < h) && rows > 1) return MARL_EINVAL;
     if ((ld_gate < d || ld_up < d) && h > 1) return MARL_EINVAL;
-    return MARL_BY_TYPE(dtype, backward, rows, d, h, x, ldx, w_gate, ld_gate, w_up, ld_up, f, p, gy, ld_gy, dx, dw_gate, dw_up, workspace_,
-                        (hipStream_t)stream);
+    const Gated g = {rows, d, h, {x, ldx, rows}, {w_gate, ld_gate, h}, {w_up, ld_up, h}};
+    return MARL_BY_TYPE(dtype, backward, g, f, p, gy, ld_gy, dx, dw_gate, dw_up, workspace_, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -133,9 +133,13 @@ Tensor3 gated_launch(const Tensor& x, const Tensor& wg, const Tensor& wu, c10::s
     if (y.numel()) {
         const Rows rx(x), rg(wg), ru(wu);
         const On on(x);
-        check(lib.marl_gated_forward(type_code(x), act_code(act), rx.n, (int32_t)wg.size(1), (int32_t)wg.size(0), rx.p(), rx.ld, rg.p(), rg.ld,
-                                     ru.p(), ru.ld, y.mutable_data_ptr(), save ? f.mutable_data_ptr() : nullptr,
-                                     save ? p.mutable_data_ptr() : nullptr, on.stream), "marl_gated_forward");
+        const int dt = type_code(x);
+        const int32_t h = (int32_t)wg.size(0), d = (int32_t)wg.size(1);
+        const size_t bytes = lib.marl_gated_workspace_bytes(dt, rx.n, d, h, rx.p(), rx.ld, rg.p(), rg.ld, ru.p(), ru.ld, 0);
+        Tensor ws = bytes ? scratch(x, bytes) : Tensor();
+        check(lib.marl_gated_forward(dt, act_code(act), rx.n, d, h, rx.p(), rx.ld, rg.p(), rg.ld, ru.p(), ru.ld, y.mutable_data_ptr(),
+                                     save ? f.mutable_data_ptr() : nullptr, save ? p.mutable_data_ptr() : nullptr,
+                                     bytes ? ws.mutable_data_ptr() : nullptr, on.stream), "marl_gated_forward");
     }
     return {y, f, p};
 }
@@ -150,7 +154,7 @@ Tensor3 gated_linear_backward(const Tensor& gy, const Tensor& x, const Tensor& w
     const Rows rx(x), rg(wg), ru(wu), rgy(gy);
     const On on(x);
     const int dt = type_code(x);
-    Tensor ws = scratch(x, lib.marl_gated_workspace_bytes(dt, rx.n, (int32_t)d, (int32_t)h));
+    Tensor ws = scratch(x, lib.marl_gated_workspace_bytes(dt, rx.n, (int32_t)d, (int32_t)h, rx.p(), rx.ld, rg.p(), rg.ld, ru.p(), ru.ld, 1));
     check(lib.marl_gated_backward(dt, rx.n, (int32_t)d, (int32_t)h, rx.p(), rx.ld, rg.p(), rg.ld, ru.p(), ru.ld, f.const_data_ptr(),
                                   p.const_data_ptr(), rgy.p(), rgy.ld, need_x ? dx.mutable_data_ptr() : nullptr,
                                   need_w ? dg.mutable_data_ptr() : nullptr, need_w ? du.mutable_data_ptr() : nullptr, ws.mutable_data_ptr(),

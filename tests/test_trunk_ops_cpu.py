@@ -66,17 +66,20 @@ def test_shapes_on_the_meta_device():
 def test_entry_points_check_their_arguments():
     lib, P = _lib.load(), 1 << 12                     # P: a pointer that is never followed
     E, U = _lib.MARL_EINVAL, _lib.MARL_EUNSUPPORTED
-    gf = lambda dt=0, act=0, rows=2, d=8, h=8, x=P, ldx=8, wg=P, ldg=8, y=P, a=None, b=None: \
-        lib.marl_gated_forward(dt, act, rows, d, h, x, ldx, wg, ldg, P, 8, y, a, b, None)
+    gf = lambda dt=0, act=0, rows=2, d=8, h=8, x=P, ldx=8, wg=P, ldg=8, y=P, a=None, b=None, ws=None: \
+        lib.marl_gated_forward(dt, act, rows, d, h, x, ldx, wg, ldg, P, 8, y, a, b, ws, None)
     for bad in (dict(dt=3), dict(dt=-1), dict(act=4), dict(rows=0), dict(d=0), dict(h=0), dict(x=None), dict(wg=None), dict(y=None),
-                dict(ldx=7), dict(ldg=7), dict(a=P)):
+                dict(ldx=7), dict(ldg=7), dict(a=P), dict(ws=P + 8), dict(rows=100, x=P + 4)):
         assert gf(**bad) == E, bad
     assert gf(rows=1 << 31) == U and gf(d=(1 << 24) + 1, ldx=1 << 25, ldg=1 << 25) == U
     gb = lambda rows=2, d=8, h=8, a=P, gy=P, ldgy=8, dx=P, dwg=P, dwu=P, ws=P: \
         lib.marl_gated_backward(0, rows, d, h, P, 8, P, 8, P, 8, a, P, gy, ldgy, dx, dwg, dwu, ws, None)
     for bad in (dict(rows=0), dict(a=None), dict(gy=None), dict(ldgy=7), dict(dwu=None), dict(ws=None), dict(ws=P + 8)):
         assert gb(**bad) == E, bad
-    assert lib.marl_gated_workspace_bytes(0, 0, 8, 8) == 0 and lib.marl_gated_workspace_bytes(1, 100, 8, 16) >= 100 * 32 * 2
+    ws = lambda dt, rows, d, h, x=P, ldx=8, backward=0: lib.marl_gated_workspace_bytes(dt, rows, d, h, x, ldx, P, ldx, P, ldx, backward)
+    assert ws(0, 0, 8, 8, backward=1) == 0 and ws(1, 100, 8, 16, backward=1) >= 100 * 32 * 2
+    assert ws(1, 100, 8, 16) == 0 and ws(1, 64, 7, 16, ldx=7) == 0 and ws(1, 100, 8, 16, x=P + 2) >= 100 * 8 * 2
+    assert ws(1, 100, 7, 16, ldx=7) >= 100 * 8 * 2 + 2 * 16 * 8 * 2
     nf = lambda dt=0, kind=0, rows=2, d=8, x=P, ldx=8, gate=None, ldg=0, eps=1e-5, stats=None: \
         lib.marl_residual_norm(dt, kind, rows, d, x, ldx, P, 8, P, P, gate, ldg, 1.0, eps, P, P, stats, None)
     for bad in (dict(dt=3), dict(kind=2), dict(rows=0), dict(d=0), dict(x=None), dict(ldx=7), dict(gate=P, ldg=7), dict(eps=-1.0),
