@@ -3,17 +3,24 @@
 //     top-k   the first k of the order             top-p   of those, the shortest prefix whose mass reaches p of theirs
 //     min-p   w_i >= min_p (of the largest)        draw    in index order, the first i with w_0 + .. + w_i > u * sum
 // The kept set is always a prefix of the order, so it is described by its last element (value, index).  Weights are
-// held as 64-bit integers, w 2^43 rounded: their sums do not depend on the order of adding, so LDS atomics and any
-// launch shape give the same index, and a row of 2^20 logits cannot overflow.  exp is evaluated in float64: an index
+// held as integers, w 2^42 rounded: their sums do not depend on the order of adding, so LDS atomics and any launch shape
+// give the same index; sums are 64-bit integers (a row of 2^20 logits cannot overflow) or, up to 2048 logits, float64, which
+// holds integers up to 2^53 exactly.  exp is evaluated in float64: an index
 // depends on which side of a border a sum of many weights falls.
 // NaN counts as -inf; +inf takes all the mass (several share it); a row without a finite or +inf logit gives index -1
 // and log-probability -inf.  temperature <= 0: the first largest logit.
-// Rows of up to 64 logits: a group of lanes per row, everything in registers.  Longer rows: a workgroup per row, which
-// reads its row a few times (the first time from HBM, then from L2): maximum; counts and masses over 2048 bins of
-// 1/64 nat below the maximum; the elements of the bin in which a border falls, sorted in LDS; the masses of the kept.
+// Rows of up to 64 logits: a group of lanes per row, everything in registers.  Up to 2048: a wave per row, likewise; the
+// borders of top-k and top-p are found by bisection over the bits of the ordered values, a count (ballots) or a sum each.
+// Longer rows: a workgroup per row, which
+// reads its row a few times (the first time from HBM, then from L2).  With a small top-k, twice: the maximum, and every
+// thread's own; k threads have a maximum above the k-th largest of those, so no element below it can be among the first k;
+// the few elements above are sorted in LDS and the rest happens there.  Otherwise: maximum; counts and masses over bins
+// of a fraction of a nat below the maximum; the elements of the bin in which a border falls, sorted in LDS; the masses of
+// the kept.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
+#include <type_traits>
 
 #include "marl_env.h"
 #include "marl_net.h"
@@ -61,11 +68,49 @@ __device__ __forceinline__ Rule rule_of(const SampleArgs& a, int64_t row) {
     return r;
 }
 
-constexpr double FIXED = 8796093022208.0;                                // 2^43
+constexpr double FIXED = 4398046511104.0;                                // 2^42
 __device__ __forceinline__ float clean(float l) { return l != l ? -HUGE_VALF : l + 0.0f; }      // NaN -> -inf, -0 -> 0
 // (l - max) / temperature, 0 for the maximum itself (also where that is infinite)
 __device__ __forceinline__ double scaled(float l, float top, double inv_t) { return l == top ? 0.0 : ((double)l - (double)top) * inv_t; }
-__device__ __forceinline__ u64 weight(double z) { return z > -31.0 ? (u64)(exp(z) * FIXED + 0.5) : 0; }
+// exp(z), z <= 0, in units of 2^-42, rounded to an integer (0 below -31 and for NaN): e^z = 2^(n / 64) e^r, |r| <= ln 2 / 128,
+// with n / 64's fraction from a table of 64 and e^r from its series up to r^5 (rest below 4e-17).  The powers of two are
+// added to the exponent; adding 1.5 2^52 rounds.  Half of the instructions of exp() and a conversion.
+__constant__ const double kPow64[64] = {
+    1.0, 1.0108892860517005, 1.0218971486541166, 1.0330248790212284,
+    1.0442737824274138, 1.0556451783605572, 1.0671404006768237, 1.0787607977571199,
+    1.0905077326652577, 1.102382583307841, 1.1143867425958924, 1.1265216186082418,
+    1.1387886347566916, 1.1511892299529827, 1.1637248587775775, 1.1763969916502812,
+    1.189207115002721, 1.202156731452703, 1.215247359980469, 1.22848053610687,
+    1.241857812073484, 1.255380757024691, 1.2690509571917332, 1.2828700160787783,
+    1.2968395546510096, 1.3109612115247644, 1.3252366431597413, 1.339667524053303,
+    1.3542555469368927, 1.3690024229745905, 1.383909881963832, 1.3989796725383112,
+    1.4142135623730951, 1.42961333839197, 1.4451808069770467, 1.460917794180647,
+    1.4768261459394993, 1.4929077282912648, 1.5091644275934228, 1.5255981507445384,
+    1.5422108254079407, 1.559004400237837, 1.5759808451078865, 1.593142151342267,
+    1.6104903319492543, 1.6280274218573478, 1.645755478153965, 1.6636765803267364,
+    1.681792830507429, 1.7001063537185235, 1.718619298122478, 1.7373338352737062,
+    1.7562521603732995, 1.7753764925265212, 1.7947090750031072, 1.8142521755003989,
+    1.8340080864093424, 1.8539791250833855, 1.8741676341103, 1.8945759815869656,
+    1.9152065613971474, 1.9360617934922943, 1.9571441241754002, 1.978456026387951
+};
+constexpr double ROUND = 6755399441055744.0;                             // 1.5 2^52
+__device__ __forceinline__ double weight_plus_round(double z, const double* pow64) {
+    z = fmax(z, -40.0);                                                  // e^-40 rounds to 0; NaN becomes -40
+    const double m = fma(z, 92.332482616893656759, ROUND);               // 64 / ln 2: the nearest integer in the low word
+    const int n = (int)(uint32_t)__double_as_longlong(m);
+    const double r = fma(m - ROUND, -0.010830424696249145, z);           // ln 2 / 64
+    double e = fma(r, 1.0 / 120.0, 1.0 / 24.0);
+    e = fma(r, e, 1.0 / 6.0);
+    e = fma(r, e, 0.5);
+    e = fma(r, e, 1.0);
+    e = fma(r, e, 1.0);
+    const long long v = __double_as_longlong(e * pow64[n & 63]) + ((long long)((n >> 6) + 42) << 52);
+    return __longlong_as_double(v) + ROUND;
+}
+__device__ __forceinline__ double weight_f64(double z, const double* pow64) { return weight_plus_round(z, pow64) - ROUND; }
+__device__ __forceinline__ u64 weight(double z, const double* pow64) {
+    return (u64)(__double_as_longlong(weight_plus_round(z, pow64)) - __double_as_longlong(ROUND));
+}
 __device__ __forceinline__ float log_prob_of(double z, u64 total) { return (float)(z - log((double)total / FIXED)); }
 
 __device__ __forceinline__ u64 shfl_u64(u64 v, int src, int width) {
@@ -91,7 +136,7 @@ __global__ __launch_bounds__(256) void sample_short_kernel(const SampleArgs a) {
     for (int o = L / 2; o > 0; o /= 2) top = fmaxf(top, __shfl_xor(top, o, L));
     const bool any = top > -HUGE_VALF;
     const double z = any ? scaled(l, top, rule.inv_t) : -HUGE_VAL;
-    u64 w = rule.greedy ? 0 : weight(z);
+    u64 w = rule.greedy || !(z > -31.0) ? 0 : (u64)(exp(z) * FIXED + 0.5);
     if (__any(rule.k > 0 || rule.p < 1.0)) {
         int rank = 0;
         u64 before = 0;
@@ -126,28 +171,197 @@ __global__ __launch_bounds__(256) void sample_short_kernel(const SampleArgs a) {
     }
 }
 
-// -- longer rows: a workgroup per row ----------------------------------------------------------------------------------
-constexpr int BINS = 2048, CAP = 2048;
-constexpr double BINS_PER_NAT = 64.0;
-
+// -- up to 64 NE logits: a wave per row, lane i holds logits NE i .. NE i + NE - 1 -------------------------------------------
 __device__ __forceinline__ uint32_t key_of(float l) {                    // larger value, larger key
     const uint32_t b = __float_as_uint(l);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-__device__ __forceinline__ int bin_of(double z) {
-    const double b = -z * BINS_PER_NAT;
+__device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key); }
+// The kept prefix of the order ends with (key, index), both included.
+struct Cut { uint32_t key, index; };
+__device__ __forceinline__ bool inside(const Cut& c, uint32_t key, uint32_t i) { return key > c.key || (key == c.key && i <= c.index); }
+
+__device__ __forceinline__ double target_of(const SampleArgs& a, int64_t r, double total) {
+    float u = a.u[r];
+    u = u > 0.0f ? (u < 1.0f ? u : 1.0f) : 0.0f;
+    const double t = (double)u * total;
+    return t < total ? t : total - 1.0;                  // u = 1, or rounded up: the last kept element
+}
+
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+    for (int o = 32; o > 0; o /= 2) v += __shfl_xor(v, o);
+    return v;
+}
+// sum over the lanes below
+__device__ __forceinline__ double wave_before(double v, int lane) {
+    double s = v;
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) { const double t = __shfl_up(s, o); if (lane >= o) s += t; }
+    return s - v;
+}
+
+template <typename T, int NE>
+__global__ __launch_bounds__(256) void sample_wave_kernel(const SampleArgs a) {
+    constexpr int CE = Chunk<T>::n;
+    __shared__ double pow64[64];
+    if (threadIdx.x < 64) pow64[threadIdx.x] = kPow64[threadIdx.x];
+    __syncthreads();
+    const int lane = threadIdx.x & 63;
+    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (r >= a.rows) return;
+    const T* row = (const T*)a.logits + r * a.ld;
+    const Rule rule = rule_of(a, r);
+    const int at = lane * NE, left = a.V - at;
+    float l[NE];
+    if constexpr (NE >= CE) {
+#pragma unroll
+        for (int c = 0; c < NE; c += CE) {
+            const Vec<T> v = load_part(row + (left > c ? at + c : 0), left - c);
+#pragma unroll
+            for (int e = 0; e < CE; ++e) l[c + e] = left > c + e ? clean(to_f32(v.e[e])) : -HUGE_VALF;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < NE; ++e) l[e] = left > e ? clean(to_f32(row[at + e])) : -HUGE_VALF;
+    }
+    float top = l[0];
+#pragma unroll
+    for (int e = 1; e < NE; ++e) top = fmaxf(top, l[e]);
+#pragma unroll
+    for (int o = 32; o > 0; o /= 2) top = fmaxf(top, __shfl_xor(top, o));
+    if (!(top > -HUGE_VALF)) {
+        if (lane == 0) { a.index[r] = -1; a.log_prob[r] = -HUGE_VALF; }
+        return;
+    }
+    if (rule.greedy) {
+        int mine = NE;
+#pragma unroll
+        for (int e = NE - 1; e >= 0; --e) if (l[e] == top) mine = e;
+        const unsigned long long any = __ballot(mine < NE);
+        if (lane == __ffsll((long long)any) - 1) { a.index[r] = at + mine; a.log_prob[r] = 0.0f; }
+        return;
+    }
+    double w[NE];
+#pragma unroll
+    for (int e = 0; e < NE; ++e) w[e] = weight_f64(scaled(l[e], top, rule.inv_t), pow64);
+    // the first `take` of the elements equal to `key`, in index order, are kept, those above all, the others lose their weight
+    auto keep = [&](uint32_t key, int take) {
+        int mine = 0;
+#pragma unroll
+        for (int e = 0; e < NE; ++e) mine += key_of(l[e]) == key;
+        int before = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o *= 2) { const int t = __shfl_up(before, o); if (lane >= o) before += t; }
+        before -= mine;
+#pragma unroll
+        for (int e = 0; e < NE; ++e) {
+            const uint32_t k = key_of(l[e]);
+            if (k < key || (k == key && before >= take)) w[e] = 0.0;
+            before += k == key;
+        }
+    };
+    constexpr int LOW = sizeof(T) == 4 ? 0 : std::is_same<T, bf16>::value ? 16 : 13;      // bits below are equal in every key of a sign
+    // keys of negative values have ones there: a candidate is compared with them all set
+    constexpr uint32_t ONES = (1u << LOW) - 1;
+    if (rule.k > 0) {
+        uint32_t key = 0;                       // the largest with at least k elements at or above it
+#pragma unroll 1
+        for (int bit = 31; bit >= LOW; --bit) {
+            const uint32_t c = key | (1u << bit);
+            int n = 0;
+#pragma unroll
+            for (int e = 0; e < NE; ++e) n += __popcll(__ballot((key_of(l[e]) | ONES) >= (c | ONES)));
+            if (n >= rule.k) key = c;
+        }
+        int above = 0;
+#pragma unroll
+        for (int e = 0; e < NE; ++e) above += __popcll(__ballot((key_of(l[e]) | ONES) > (key | ONES)));
+        keep(key & 0x80000000u ? key : key | ONES, rule.k - above);
+    }
+    if (rule.p < 1.0) {
+        double sum = 0.0;
+#pragma unroll
+        for (int e = 0; e < NE; ++e) sum += w[e];
+        double goal = rule.p * wave_sum(sum);
+        goal = goal > 1.0 ? goal : 1.0;
+        uint32_t key = 0;                       // the largest with a mass of at least `goal` at or above it
+#pragma unroll 1
+        for (int bit = 31; bit >= LOW; --bit) {
+            const uint32_t c = key | (1u << bit);
+            double m = 0.0;
+#pragma unroll
+            for (int e = 0; e < NE; ++e) m += (key_of(l[e]) | ONES) >= (c | ONES) ? w[e] : 0.0;
+            if (wave_sum(m) >= goal) key = c;
+        }
+        double above = 0.0, each_ = 0.0;
+#pragma unroll
+        for (int e = 0; e < NE; ++e) {
+            const uint32_t k = key_of(l[e]) | ONES;
+            above += k > (key | ONES) ? w[e] : 0.0;
+            if (k == (key | ONES)) each_ = fmax(each_, w[e]);
+        }
+        above = wave_sum(above);
+#pragma unroll
+        for (int o = 32; o > 0; o /= 2) each_ = fmax(each_, __shfl_xor(each_, o));
+        // the smallest number of them that reaches the goal (at least one)
+        double take = ceil((goal - above) / each_);
+        if (take > 1.0 && above + (take - 1.0) * each_ >= goal) take -= 1.0;
+        if (above + take * each_ < goal) take += 1.0;
+        keep(key & 0x80000000u ? key : key | ONES, take > 1.0 ? (int)fmin(take, 4096.0) : 1);
+    }
+    double sum = 0.0;
+#pragma unroll
+    for (int e = 0; e < NE; ++e) {
+        if (scaled(l[e], top, rule.inv_t) < rule.log_m) w[e] = 0.0;
+        sum += w[e];
+    }
+    double run = wave_before(sum, lane);
+    const double total = __shfl(run + sum, 63), target = target_of(a, r, total);
+    if (run <= target && run + sum > target) {
+        bool found = false;
+#pragma unroll
+        for (int e = 0; e < NE; ++e) {
+            run += w[e];
+            if (!found && run > target) {
+                found = true;
+                a.index[r] = at + e;
+                a.log_prob[r] = log_prob_of(scaled(l[e], top, rule.inv_t), (u64)total);
+            }
+        }
+    }
+}
+
+// -- longer rows: a workgroup per row ----------------------------------------------------------------------------------
+// The workgroups: 1024 threads for the longest rows (one or two to a CU); 256 with a quarter of the LDS for shorter ones.
+template <int THREADS> struct Dim {
+    static constexpr int BINS = THREADS == 1024 ? 2048 : 512, CAP = BINS;        // bins; elements sorted at once
+    static constexpr double PER_NAT = BINS / 32.0;                               // the bins cover 32 nats
+};
+
+template <int THREADS> __device__ __forceinline__ int bin_of(double z) {
+    constexpr int BINS = Dim<THREADS>::BINS;
+    const double b = -z * Dim<THREADS>::PER_NAT;
     return b < (double)(BINS - 1) ? (int)b : BINS - 1;
 }
 
+// A float32 bound of the logits in bins up to `bin`: those of later bins lie below it, or so little above that the bin
+// itself has to be looked at (a step of float32 lower than the edge, for the rounding on the way).
+template <int THREADS> __device__ __forceinline__ float lower_edge(int bin, float top, double inv_t) {
+    if (bin >= Dim<THREADS>::BINS - 1) return -HUGE_VALF;
+    const float edge = (float)((double)top - (double)(bin + 1) / (Dim<THREADS>::PER_NAT * inv_t));
+    return edge - fabsf(edge) * 0x1p-22f - 0x1p-126f;
+}
+
 template <int THREADS> struct Shared {
-    uint32_t count[BINS];
-    u64 mass[BINS];
-    u64 list[CAP];                  // (~key << 32 | index): ascending = the order of the row
+    double pow64[64];
+    u64 mass[Dim<THREADS>::BINS];
+    u64 list[Dim<THREADS>::CAP];    // (~key << 32 | index): ascending = the order of the row
+    uint32_t count[Dim<THREADS>::BINS];
     u64 wave64[THREADS / 64];
     uint32_t wave32[THREADS / 64];
-    u64 found_mass, found64;
+    u64 found_mass;
     uint32_t n, found, found_count;
-    float top;
 };
 
 // inclusive scan over the workgroup; *total = the sum
@@ -165,14 +379,21 @@ template <int THREADS> __device__ __forceinline__ u64 block_scan(u64 v, Shared<T
     return v + before;
 }
 
-// The kept prefix of the order ends with (key, index), both included.
-struct Cut { uint32_t key, index; };
-__device__ __forceinline__ bool inside(const Cut& c, uint32_t key, uint32_t i) { return key > c.key || (key == c.key && i <= c.index); }
-
+// f(index, value) for every element of the row, four chunks per thread under way at a time
 template <typename T, int THREADS, class F>
 __device__ __forceinline__ void each(const T* row, int32_t V, F&& f) {
-    constexpr int CE = Chunk<T>::n;
-    for (int32_t c = threadIdx.x * CE; c < V; c += THREADS * CE) {
+    constexpr int CE = Chunk<T>::n, TURN = THREADS * CE;
+    int32_t c = threadIdx.x * CE;
+    for (; c + 3 * TURN + CE <= V; c += 4 * TURN) {
+        Vec<T> v[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = load_chunk(row + c + q * TURN);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int e = 0; e < CE; ++e) f(c + q * TURN + e, clean(to_f32(v[q].e[e])));
+    }
+    for (; c < V; c += TURN) {
         const Vec<T> v = load_part(row + c, (int64_t)V - c);
 #pragma unroll
         for (int e = 0; e < CE; ++e) if (c + e < V) f(c + e, clean(to_f32(v.e[e])));
@@ -180,10 +401,10 @@ __device__ __forceinline__ void each(const T* row, int32_t V, F&& f) {
 }
 
 // Where the running sum over the bins (counts, or masses) reaches `goal` first: the bin, and the count and mass before
-// it.  by_count: first bin with count(0..b) >= goal_n; else the last bin with mass before it < goal_m (and not empty).
+// it.  by_count: first bin with count(0..b) >= goal_n; else the last bin of any mass with less than goal_m before it.
 template <int THREADS>
 __device__ __forceinline__ void find_bin(Shared<THREADS>& s, bool by_count, uint32_t goal_n, double goal_m, uint32_t& bin, uint32_t& n_before, u64& m_before) {
-    constexpr int PER = BINS / THREADS;
+    constexpr int PER = Dim<THREADS>::BINS / THREADS;
     u64 n = 0, m = 0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) { n += s.count[threadIdx.x * PER + i]; m += s.mass[threadIdx.x * PER + i]; }
@@ -197,7 +418,7 @@ __device__ __forceinline__ void find_bin(Shared<THREADS>& s, bool by_count, uint
     for (int i = 0; i < PER; ++i) {
         const int b = threadIdx.x * PER + i;
         const uint32_t c = s.count[b];
-        const bool here = by_count ? an < goal_n && an + c >= goal_n : c > 0 && (double)am < goal_m;
+        const bool here = by_count ? an < goal_n && an + c >= goal_n : s.mass[b] > 0 && (double)am < goal_m;
         if (here) atomicMax(&s.found, (uint32_t)b);
         an += c; am += s.mass[b];
     }
@@ -215,21 +436,45 @@ __device__ __forceinline__ void find_bin(Shared<THREADS>& s, bool by_count, uint
     __syncthreads();
 }
 
+// ascending order of the first n elements of the list
+template <int THREADS> __device__ __forceinline__ void sort_list(Shared<THREADS>& s, int n) {
+    int size = 64;
+    while (size < n) size *= 2;
+    for (int i = threadIdx.x; i < size; i += THREADS) if (i >= n) s.list[i] = ~0ull;
+    for (int k = 2; k <= size; k *= 2)
+        for (int j = k / 2; j > 0; j /= 2) {
+            __syncthreads();
+            for (int i = threadIdx.x; i < size / 2; i += THREADS) {
+                const int x = 2 * j * (i / j) + i % j, y = x + j;
+                const u64 p = s.list[x], q = s.list[y];
+                if ((p > q) == ((x & k) == 0)) { s.list[x] = q; s.list[y] = p; }
+            }
+        }
+    __syncthreads();
+}
+
 // The last element of the shortest prefix of the order that holds goal_n elements (by_count), or that cannot lose its
 // last element without its mass falling below goal_m, among the elements of linear bin `bin`; *mass = the mass up to
 // and with it.  Elements of one bin are sorted in LDS; a bin with more than fits is cut by its keys first, down to a
 // single value if need be, whose elements count by index.
 template <typename T, int THREADS>
-__device__ Cut resolve(Shared<THREADS>& s, const T* row, int32_t V, float top, double inv_t, uint32_t bin, bool by_count, uint32_t goal_n, double goal_m,
-                       uint32_t n_before, u64 m_before, u64* mass) {
+__device__ __noinline__ Cut resolve(Shared<THREADS>& s, const T* row, int32_t V, float top, double inv_t, uint32_t bin, bool by_count, uint32_t goal_n, double goal_m,
+                                    uint32_t n_before, u64 m_before, u64* mass) {
+    constexpr int BINS = Dim<THREADS>::BINS, CAP = Dim<THREADS>::CAP;
     uint32_t lo = 0, hi = 0xFFFFFFFFu;
+    // cheap bounds first: most of the row is outside of the bin (+inf logits, whose distances are not numbers: no bounds)
+    const bool bounded = fabsf(top) < HUGE_VALF;
+    const float floor_ = bounded ? lower_edge<THREADS>((int)bin, top, inv_t) : -HUGE_VALF;
+    const float edge = (float)((double)top - (double)bin / (Dim<THREADS>::PER_NAT * inv_t));
+    const float ceiling = bounded && bin > 0 ? edge + fabsf(edge) * 0x1p-22f + 0x1p-126f : HUGE_VALF;
     for (;;) {
-        if (threadIdx.x == 0) { s.n = 0; s.found64 = ((u64)0) ; s.found = 0xFFFFFFFFu; s.found_count = 0; }
+        if (threadIdx.x == 0) { s.n = 0; s.found = 0xFFFFFFFFu; s.found_count = 0; }
         __syncthreads();
         uint32_t kmin = 0xFFFFFFFFu, kmax = 0, mine = 0;
         each<T, THREADS>(row, V, [&](int32_t i, float l) {
+            if (!(l >= floor_ && l <= ceiling)) return;
             const uint32_t key = key_of(l);
-            if (key < lo || key > hi || !(l > -HUGE_VALF) || bin_of(scaled(l, top, inv_t)) != (int)bin) return;
+            if (key < lo || key > hi || !(l > -HUGE_VALF) || bin_of<THREADS>(scaled(l, top, inv_t)) != (int)bin) return;
             kmin = key < kmin ? key : kmin; kmax = key > kmax ? key : kmax; ++mine;
             const uint32_t at = atomicAdd(&s.n, 1u);
             if (at < CAP) s.list[at] = ((u64)(uint32_t)~key << 32) | (uint32_t)i;
@@ -240,58 +485,40 @@ __device__ Cut resolve(Shared<THREADS>& s, const T* row, int32_t V, float top, d
         kmin = s.found; kmax = s.found_count;
         __syncthreads();
         if (n <= CAP) {
-            int size = 64;
-            while (size < (int)n) size *= 2;
-            for (int i = threadIdx.x; i < size; i += THREADS) if (i >= (int)n) s.list[i] = ~0ull;
-            for (int k = 2; k <= size; k *= 2)
-                for (int j = k / 2; j > 0; j /= 2) {
-                    __syncthreads();
-                    for (int i = threadIdx.x; i < size / 2; i += THREADS) {
-                        const int x = 2 * j * (i / j) + i % j, y = x + j;
-                        const u64 p = s.list[x], q = s.list[y];
-                        if ((p > q) == ((x & k) == 0)) { s.list[x] = q; s.list[y] = p; }
-                    }
-                }
-            __syncthreads();
+            sort_list<THREADS>(s, (int)n);
             // mass before and up to every element, in order: each thread a run of them
             constexpr int PER = CAP / THREADS;
             u64 w[PER], sum = 0;
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
                 const int at = threadIdx.x * PER + i;
-                uint32_t key = at < (int)n ? ~(uint32_t)(s.list[at] >> 32) : 0;
-                const float l = __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
-                w[i] = at < (int)n ? weight(scaled(l, top, inv_t)) : 0;
+                w[i] = at < (int)n ? weight(scaled(value_of(~(uint32_t)(s.list[at] >> 32)), top, inv_t), s.pow64) : 0;
                 sum += w[i];
             }
             u64 total;
             u64 run = m_before + block_scan<THREADS>(sum, s, &total) - sum;
             if (threadIdx.x == 0) s.found = 0;
             __syncthreads();
+            u64 upto[PER];
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
                 const uint32_t at = threadIdx.x * PER + i;
-                const bool in = at < n && (by_count ? n_before + at < goal_n : n_before + at == 0 || (double)run < goal_m);
+                const bool in = at < n && (by_count ? n_before + at < goal_n : at == 0 || (double)run < goal_m);
                 if (in) atomicMax(&s.found, at);
-                run += w[i];
+                upto[i] = run += w[i];
             }
             __syncthreads();
             const uint32_t last = s.found;
-            run = m_before + block_scan<THREADS>(sum, s, &total) - sum;
 #pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                run += w[i];
-                if ((uint32_t)(threadIdx.x * PER + i) == last) s.found_mass = run;
-            }
+            for (int i = 0; i < PER; ++i) if ((uint32_t)(threadIdx.x * PER + i) == last) s.found_mass = upto[i];
             __syncthreads();
             *mass = s.found_mass;
             const u64 e = s.list[last];
             __syncthreads();
             return Cut{~(uint32_t)(e >> 32), (uint32_t)e};
         }
-        const float l_hi = __uint_as_float(kmax & 0x80000000u ? kmax & 0x7FFFFFFFu : ~kmax);
         if (kmin == kmax) {                         // one value: `take` of its elements, in index order
-            const u64 w = weight(scaled(l_hi, top, inv_t));
+            const u64 w = weight(scaled(value_of(kmax), top, inv_t), s.pow64);
             uint32_t take;
             if (by_count) take = goal_n - n_before;
             else {                                  // smallest t with m_before + t w >= goal_m
@@ -325,13 +552,14 @@ __device__ Cut resolve(Shared<THREADS>& s, const T* row, int32_t V, float top, d
         for (int b = threadIdx.x; b < BINS; b += THREADS) { s.count[b] = 0; s.mass[b] = 0; }
         __syncthreads();
         each<T, THREADS>(row, V, [&](int32_t, float l) {
+            if (!(l >= floor_ && l <= ceiling)) return;
             const uint32_t key = key_of(l);
             if (key < kmin || key > kmax || !(l > -HUGE_VALF)) return;
             const double z = scaled(l, top, inv_t);
-            if (bin_of(z) != (int)bin) return;
+            if (bin_of<THREADS>(z) != (int)bin) return;
             const int b = (int)((kmax - key) >> shift);
             atomicAdd(&s.count[b], 1u);
-            atomicAdd(&s.mass[b], weight(z));
+            atomicAdd(&s.mass[b], weight(z, s.pow64));
         });
         __syncthreads();
         uint32_t b, nb;
@@ -344,6 +572,152 @@ __device__ Cut resolve(Shared<THREADS>& s, const T* row, int32_t V, float top, d
     }
 }
 
+// counts, masses or both of the row over the linear bins
+template <typename T, int THREADS>
+__device__ __noinline__ void histogram(Shared<THREADS>& s, const T* row, int32_t V, float top, double inv_t, bool counts, bool masses) {
+    for (int b = threadIdx.x; b < Dim<THREADS>::BINS; b += THREADS) { s.count[b] = 0; s.mass[b] = 0; }
+    __syncthreads();
+    each<T, THREADS>(row, V, [&](int32_t, float l) {
+        if (!(l > -HUGE_VALF)) return;
+        const double z = scaled(l, top, inv_t);
+        const int b = bin_of<THREADS>(z);
+        if (counts) atomicAdd(&s.count[b], 1u);
+        if (masses) { const u64 w = weight(z, s.pow64); if (w) atomicAdd(&s.mass[b], w); }
+    });
+    __syncthreads();
+}
+
+// where the kept prefix ends under top-k and top-p
+template <typename T, int THREADS>
+__device__ __noinline__ Cut cut_of(Shared<THREADS>& s, const T* row, int32_t V, float top, const Rule& rule) {
+    Cut cut = {0, 0xFFFFFFFFu};
+    histogram<T, THREADS>(s, row, V, top, rule.inv_t, rule.k > 0, rule.p < 1.0);
+    u64 finite = 0, total = 0;
+    for (int b = threadIdx.x; b < Dim<THREADS>::BINS; b += THREADS) { finite += s.count[b]; total += s.mass[b]; }
+    block_scan<THREADS>(finite, s, &finite);
+    block_scan<THREADS>(total, s, &total);
+    uint32_t b, nb;
+    u64 mb;
+    if (rule.k > 0 && (u64)rule.k < finite) {
+        find_bin<THREADS>(s, true, (uint32_t)rule.k, 0.0, b, nb, mb);
+        const bool fits = s.count[b] <= Dim<THREADS>::CAP;              // else resolve() overwrites the bins
+        cut = resolve<T, THREADS>(s, row, V, top, rule.inv_t, b, true, (uint32_t)rule.k, 0.0, nb, mb, &total);
+        if (rule.p < 1.0 && !fits) histogram<T, THREADS>(s, row, V, top, rule.inv_t, false, true);
+    }
+    if (rule.p < 1.0) {
+        const double goal = rule.p * (double)total;
+        find_bin<THREADS>(s, false, 0, goal > 1.0 ? goal : 1.0, b, nb, mb);
+        u64 m;
+        // (counts may be absent or stale here: resolve() needs none, its bin has less than `goal` before it)
+        const Cut c = resolve<T, THREADS>(s, row, V, top, rule.inv_t, b, false, 0, goal, 0, mb, &m);
+        if (c.key > cut.key || (c.key == cut.key && c.index < cut.index)) cut = c;
+    }
+    return cut;
+}
+
+// Rows with top-k up to CAP / 4: true if the draw was made.  `mine`: the thread's own maximum.
+template <typename T, int THREADS>
+__device__ __forceinline__ bool draw_from_first_k(Shared<THREADS>& s, const SampleArgs& a, int64_t r, const T* row, float top, float mine, const Rule& rule) {
+    constexpr int BINS = Dim<THREADS>::BINS, CAP = Dim<THREADS>::CAP, PER = CAP / THREADS;
+    const int32_t V = a.V;
+    for (int b = threadIdx.x; b < BINS; b += THREADS) { s.count[b] = 0; s.mass[b] = 0; }
+    if (threadIdx.x == 0) { s.n = 0; s.found = BINS; }
+    __syncthreads();
+    if (mine > -HUGE_VALF) atomicAdd(&s.count[bin_of<THREADS>(scaled(mine, top, rule.inv_t))], 1u);
+    __syncthreads();
+    {   // the bin of the k-th largest thread maximum
+        u64 n = 0, all;
+#pragma unroll
+        for (int i = 0; i < BINS / THREADS; ++i) n += s.count[threadIdx.x * (BINS / THREADS) + i];
+        u64 before = block_scan<THREADS>(n, s, &all) - n;
+#pragma unroll
+        for (int i = 0; i < BINS / THREADS; ++i) {
+            const uint32_t b = threadIdx.x * (BINS / THREADS) + i, c = s.count[b];
+            if (before < (u64)rule.k && before + c >= (u64)rule.k) s.found = b;
+            before += c;
+        }
+    }
+    __syncthreads();
+    const uint32_t bin = s.found;
+    if (bin >= BINS - 1) return false;              // fewer than k maxima, or in the last bin, which has no lower edge
+    // no element of bins 0 .. bin lies below this
+    const float limit = lower_edge<THREADS>(bin, top, rule.inv_t);
+    each<T, THREADS>(row, V, [&](int32_t i, float l) {
+        if (l >= limit) {
+            const uint32_t at = atomicAdd(&s.n, 1u);
+            if (at < CAP) s.list[at] = ((u64)(uint32_t)~key_of(l) << 32) | (uint32_t)i;
+        }
+    });
+    __syncthreads();
+    const int n = (int)s.n;
+    if (n > CAP) return false;
+    sort_list<THREADS>(s, n);
+    const int first = n < rule.k ? n : rule.k;
+    uint32_t index[PER];
+    double z[PER];
+    u64 w[PER], sum = 0, all;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int at = threadIdx.x * PER + i;
+        const u64 e = at < first ? s.list[at] : 0;
+        index[i] = (uint32_t)e;
+        z[i] = at < first ? scaled(value_of(~(uint32_t)(e >> 32)), top, rule.inv_t) : -HUGE_VAL;
+        w[i] = weight(z[i], s.pow64);
+        sum += w[i];
+    }
+    u64 before = block_scan<THREADS>(sum, s, &all) - sum;
+    const double goal = rule.p * (double)all;
+    sum = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const u64 own = w[i];
+        if ((rule.p < 1.0 && threadIdx.x * PER + i > 0 && !((double)before < goal)) || z[i] < rule.log_m) w[i] = 0;
+        before += own;
+        sum += w[i];
+    }
+    // index order: masses by ranges of indices (s.mass is clear), then inside the range of the draw
+    const uint32_t width = (uint32_t)(V + BINS - 1) / BINS;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) if (w[i]) atomicAdd(&s.mass[index[i] / width], w[i]);
+    if (threadIdx.x == 0) s.n = 0;
+    __syncthreads();
+    u64 m = 0, total;
+#pragma unroll
+    for (int i = 0; i < BINS / THREADS; ++i) m += s.mass[threadIdx.x * (BINS / THREADS) + i];
+    u64 run = block_scan<THREADS>(m, s, &total) - m;
+    const double target = target_of(a, r, (double)total);
+#pragma unroll
+    for (int i = 0; i < BINS / THREADS; ++i) {
+        const uint32_t b = threadIdx.x * (BINS / THREADS) + i;
+        const u64 c = s.mass[b];
+        if ((double)run <= target && (double)(run + c) > target) { s.found = b; s.found_mass = run; }
+        run += c;
+    }
+    __syncthreads();
+    const uint32_t range = s.found;
+    const u64 at_range = s.found_mass;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+        if (w[i] && index[i] / width == range) {
+            const uint32_t at = atomicAdd(&s.n, 1u);
+            s.list[at] = index[i];
+            s.mass[at] = w[i];
+        }
+    __syncthreads();
+    const int in_range = (int)s.n;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+        if (w[i] && index[i] / width == range) {
+            u64 low = at_range;
+            for (int j = 0; j < in_range; ++j) if (s.list[j] < index[i]) low += s.mass[j];
+            if ((double)low <= target && (double)(low + w[i]) > target) {
+                a.index[r] = index[i];
+                a.log_prob[r] = log_prob_of(z[i], total);
+            }
+        }
+    return true;
+}
+
 template <typename T, int THREADS>
 __global__ __launch_bounds__(THREADS) void sample_row_kernel(const SampleArgs a) {
     __shared__ Shared<THREADS> s;
@@ -353,9 +727,11 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(const SampleArgs a)
     const T* row = (const T*)a.logits + r * a.ld;
     const int32_t V = a.V;
     const Rule rule = rule_of(a, r);
+    if (threadIdx.x < 64) s.pow64[threadIdx.x] = kPow64[threadIdx.x];
     // maximum
-    float top = -HUGE_VALF;
-    each<T, THREADS>(row, V, [&](int32_t, float l) { top = fmaxf(top, l); });
+    float mine = -HUGE_VALF;
+    each<T, THREADS>(row, V, [&](int32_t, float l) { mine = fmaxf(mine, l); });
+    float top = mine;
 #pragma unroll
     for (int o = 32; o > 0; o /= 2) top = fmaxf(top, __shfl_xor(top, o));
     if (lane == 0) s.wave32[wave] = __float_as_uint(top);
@@ -377,67 +753,45 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(const SampleArgs a)
         if (threadIdx.x == 0) { a.index[r] = s.found; a.log_prob[r] = 0.0f; }
         return;
     }
-    Cut cut = {0, 0xFFFFFFFFu};
-    if (rule.k > 0 || rule.p < 1.0) {
-        for (int b = threadIdx.x; b < BINS; b += THREADS) { s.count[b] = 0; s.mass[b] = 0; }
+    if (rule.k > 0 && rule.k <= Dim<THREADS>::CAP / 4 && fabsf(top) < HUGE_VALF) {
+        if (draw_from_first_k<T, THREADS>(s, a, r, row, top, mine, rule)) return;
         __syncthreads();
-        u64 total = 0;
-        each<T, THREADS>(row, V, [&](int32_t, float l) {
-            if (!(l > -HUGE_VALF)) return;
-            const double z = scaled(l, top, rule.inv_t);
-            const int b = bin_of(z);
-            atomicAdd(&s.count[b], 1u);
-            if (rule.p < 1.0) { const u64 w = weight(z); if (w) atomicAdd(&s.mass[b], w); }
-        });
-        __syncthreads();
-        u64 finite = 0, sum = 0;
-        for (int b = threadIdx.x; b < BINS; b += THREADS) { finite += s.count[b]; sum += s.mass[b]; }
-        block_scan<THREADS>(finite, s, &finite);
-        block_scan<THREADS>(sum, s, &total);
-        uint32_t b, nb;
-        u64 mb;
-        const bool limited = rule.k > 0 && (u64)rule.k < finite;
-        if (limited) {
-            find_bin<THREADS>(s, true, (uint32_t)rule.k, 0.0, b, nb, mb);
-            // the bins may be needed again for top-p: resolve overwrites them only if the bin does not fit
-            const bool fits = s.count[b] <= CAP;
-            if (rule.p < 1.0 && !fits) {
-                cut = resolve<T, THREADS>(s, row, V, top, rule.inv_t, b, true, (uint32_t)rule.k, 0.0, nb, mb, &total);
-                for (int i = threadIdx.x; i < BINS; i += THREADS) { s.count[i] = 0; s.mass[i] = 0; }
-                __syncthreads();
-                each<T, THREADS>(row, V, [&](int32_t, float l) {
-                    if (!(l > -HUGE_VALF)) return;
-                    const double z = scaled(l, top, rule.inv_t);
-                    atomicAdd(&s.count[bin_of(z)], 1u);
-                    const u64 w = weight(z);
-                    if (w) atomicAdd(&s.mass[bin_of(z)], w);
-                });
-                __syncthreads();
-            } else {
-                cut = resolve<T, THREADS>(s, row, V, top, rule.inv_t, b, true, (uint32_t)rule.k, 0.0, nb, mb, &total);
-            }
-        }
-        if (rule.p < 1.0) {
-            const double goal = rule.p * (double)total;
-            find_bin<THREADS>(s, false, 0, goal > 1.0 ? goal : 1.0, b, nb, mb);
-            u64 m;
-            const Cut c = resolve<T, THREADS>(s, row, V, top, rule.inv_t, b, false, 0, goal, nb, mb, &m);
-            if (c.key > cut.key || (c.key == cut.key && c.index < cut.index)) cut = c;
-        }
     }
+    const Cut cut = rule.k > 0 || rule.p < 1.0 ? cut_of<T, THREADS>(s, row, V, top, rule) : Cut{0, 0xFFFFFFFFu};
     // masses of the kept elements: wave w sums its run of the row, then the whole workgroup looks into the run of the draw
-    auto kept = [&](int32_t i, float l, double z) { return l > -HUGE_VALF && !(z < rule.log_m) && inside(cut, key_of(l), (uint32_t)i); };
+    auto kept_weight = [&](int32_t i, float l) -> u64 {
+        if (!(l > -HUGE_VALF) || !inside(cut, key_of(l), (uint32_t)i)) return 0;
+        const double z = scaled(l, top, rule.inv_t);
+        return z < rule.log_m ? 0 : weight(z, s.pow64);
+    };
     constexpr int WAVES = THREADS / 64;
     const int32_t run = (V + WAVES * 64 * CE - 1) / (WAVES * 64 * CE) * (64 * CE);
     u64 sum = 0;
-    for (int32_t c = wave * run + lane * CE; c < (wave + 1) * run && c < V; c += 64 * CE) {
-        const Vec<T> v = load_part(row + c, (int64_t)V - c);
+    if (cut.key == 0 && !(rule.log_m > -HUGE_VAL) && fabsf(top) < HUGE_VALF) {       // nothing is filtered
+        double part = 0.0;                        // exact: at most 2^10 weights of at most 2^42
+        const int32_t stop = (wave + 1) * run < V ? (wave + 1) * run : V;
+        int32_t c = wave * run + lane * CE;
+        for (; c + 192 * CE + CE <= stop; c += 256 * CE) {
+            Vec<T> v[4];
 #pragma unroll
-        for (int e = 0; e < CE; ++e) {
-            if (c + e >= V) continue;
-            const float l = clean(to_f32(v.e[e]));
-            const double z = scaled(l, top, rule.inv_t);
-            if (kept(c + e, l, z)) sum += weight(z);
+            for (int q = 0; q < 4; ++q) v[q] = load_chunk(row + c + 64 * CE * q);
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int e = 0; e < CE; ++e) part += weight_f64(((double)clean(to_f32(v[q].e[e])) - (double)top) * rule.inv_t, s.pow64);
+        }
+        for (; c < stop; c += 64 * CE) {
+            const Vec<T> v = load_part(row + c, (int64_t)V - c);
+#pragma unroll
+            for (int e = 0; e < CE; ++e) if (c + e < V) part += weight_f64(((double)clean(to_f32(v.e[e])) - (double)top) * rule.inv_t, s.pow64);
+        }
+        sum = (u64)part;
+    } else {
+        for (int32_t c = wave * run + lane * CE; c < (wave + 1) * run && c < V; c += 64 * CE) {
+            const Vec<T> v = load_part(row + c, (int64_t)V - c);
+#pragma unroll
+            for (int e = 0; e < CE; ++e)
+                if (c + e < V) sum += kept_weight(c + e, clean(to_f32(v.e[e])));
         }
     }
 #pragma unroll
@@ -450,10 +804,7 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(const SampleArgs a)
     int which = 0;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) total += s.wave64[w];
-    float u = a.u[r];
-    u = u > 0.0f ? (u < 1.0f ? u : 1.0f) : 0.0f;
-    double target = (double)u * (double)total;
-    if (!(target < (double)total)) target = (double)(total - 1);          // u = 1, or rounded up: the last kept element
+    const double target = target_of(a, r, (double)total);
     {
         u64 cum = 0;
         bool hit = false;
@@ -476,24 +827,17 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(const SampleArgs a)
         const Vec<T> v = load_part(row + (c < end ? c : begin), c < end ? (int64_t)end - c : 0);
 #pragma unroll
         for (int e = 0; e < CE; ++e) {
-            w[e] = 0;
-            if (c + e < end) {
-                const float l = clean(to_f32(v.e[e]));
-                const double z = scaled(l, top, rule.inv_t);
-                if (kept(c + e, l, z)) w[e] = weight(z);
-            }
+            w[e] = c + e < end ? kept_weight(c + e, clean(to_f32(v.e[e]))) : 0;
             part += w[e];
         }
         u64 tile;
         u64 cum = before + block_scan<THREADS>(part, s, &tile) - part;
         uint32_t first = 0xFFFFFFFFu, last = 0;
 #pragma unroll
-        for (int e = CE - 1; e >= 0; --e) {
-            u64 up = cum;
-#pragma unroll
-            for (int q = 0; q <= e; ++q) up += w[q];
-            if (w[e] && (double)up > target) first = (uint32_t)(c + e);
-            if (w[e] && last == 0) last = (uint32_t)(c + e) + 1;
+        for (int e = 0; e < CE; ++e) {
+            cum += w[e];
+            if (w[e] && first == 0xFFFFFFFFu && (double)cum > target) first = (uint32_t)(c + e);
+            if (w[e]) last = (uint32_t)(c + e) + 1;
         }
         if (first != 0xFFFFFFFFu) atomicMin(&s.found, first);
         if (last) atomicMax(&s.found_count, last);
@@ -517,7 +861,14 @@ template <typename T> int run(const SampleArgs& a, hipStream_t stream) {
     else if (a.V <= 32) MARL_SHORT(32);
     else if (a.V <= 64) MARL_SHORT(64);
 #undef MARL_SHORT
-    else if (a.V <= 4096) hipLaunchKernelGGL((sample_row_kernel<T, 256>), dim3((unsigned)a.rows), dim3(256), 0, stream, a);
+#define MARL_WAVE(NE) hipLaunchKernelGGL((sample_wave_kernel<T, NE>), dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, stream, a)
+    else if (a.V <= 128) MARL_WAVE(2);
+    else if (a.V <= 256) MARL_WAVE(4);
+    else if (a.V <= 512) MARL_WAVE(8);
+    else if (a.V <= 1024) MARL_WAVE(16);
+    else if (a.V <= 2048) MARL_WAVE(32);
+#undef MARL_WAVE
+    else if (a.V <= 8192) hipLaunchKernelGGL((sample_row_kernel<T, 256>), dim3((unsigned)a.rows), dim3(256), 0, stream, a);
     else hipLaunchKernelGGL((sample_row_kernel<T, 1024>), dim3((unsigned)a.rows), dim3(1024), 0, stream, a);
     const hipError_t err = hipGetLastError();
     if (err == hipSuccess) return MARL_OK;
