@@ -21,8 +21,9 @@ using namespace marl_types;
 constexpr int GROUP = 8;                 // columns of one Philox call
 
 // One group of eight columns per thread and turn.  magic = floor(2^32 / groups): q = umulhi(i, magic) is i / groups or
-// one less, which the remainder shows.
-template <typename T>
+// one less, which the remainder shows.  WHOLE: rows of whole groups; the loads then do not branch and are under way while the
+// generator runs.
+template <typename T, bool WHOLE>
 __global__ __launch_bounds__(256) void keyed_dropout_kernel(const T* __restrict__ x, int64_t ldx, T* __restrict__ y, const int64_t* __restrict__ keys,
                                                              int64_t first_row, uint32_t total, uint32_t groups, uint32_t magic, int32_t d,
                                                              uint32_t threshold, float scale, uint32_t seed_lo, uint32_t seed_hi) {
@@ -36,7 +37,7 @@ __global__ __launch_bounds__(256) void keyed_dropout_kernel(const T* __restrict_
         T* py = y + r * d + c;
         Vec<T> v[CHUNKS];
 #pragma unroll
-        for (int k = 0; k < CHUNKS; ++k) v[k] = load_part(px + k * CE, (int64_t)d - c - k * CE);
+        for (int k = 0; k < CHUNKS; ++k) v[k] = WHOLE ? load_chunk(px + k * CE) : load_part(px + k * CE, (int64_t)d - c - k * CE);
         const uint64_t key = keys ? (uint64_t)keys[r] : (uint64_t)r;
         uint32_t w[4];
         marl_rng::philox4x32(g, marl_rng::STREAM_DROPOUT, (uint32_t)key, (uint32_t)(key >> 32), seed_lo, seed_hi, w);
@@ -48,7 +49,8 @@ __global__ __launch_bounds__(256) void keyed_dropout_kernel(const T* __restrict_
                 const uint32_t u = (col & 1) ? w[col / 2] >> 16 : w[col / 2] & 0xFFFFu;
                 v[k].e[e] = u >= threshold ? from_f32<T>(to_f32(v[k].e[e]) * scale) : (T)0.0f;
             }
-            store_part(py + k * CE, v[k], (int64_t)d - c - k * CE);
+            if (WHOLE) store_chunk(py + k * CE, v[k]);
+            else store_part(py + k * CE, v[k], (int64_t)d - c - k * CE);
         }
     }
 }
@@ -63,7 +65,8 @@ int run(int64_t rows, int32_t d, const void* x, int64_t ldx, void* y, const int6
         const int64_t n = rows - first < per_launch ? rows - first : per_launch;
         const uint32_t total = (uint32_t)n * groups;
         const uint32_t blocks = (total + 255) / 256;
-        hipLaunchKernelGGL(keyed_dropout_kernel<T>, dim3(blocks < 16384 ? blocks : 16384), dim3(256), 0, stream, (const T*)x, ldx, (T*)y, keys,
+        auto* kernel = d % GROUP == 0 ? keyed_dropout_kernel<T, true> : keyed_dropout_kernel<T, false>;
+        hipLaunchKernelGGL(kernel, dim3(blocks < 16384 ? blocks : 16384), dim3(256), 0, stream, (const T*)x, ldx, (T*)y, keys,
                            first, total, groups, magic, d, threshold, scale, (uint32_t)seed, (uint32_t)(seed >> 32));
     }
     const hipError_t err = hipGetLastError();

@@ -4,8 +4,10 @@
 // one value per channel or one per element.  Backward, with hats for the normalised values, t = gy + N'(gn w_pre; y):
 //     dx = scale t,  dgate = t o,  dblock = N'(t gate w_post; block),  dw_post = sum t gate block^,  dw_pre = sum gn y^,
 //     N'(g; v) = r (g - mean(g) [layer only] - v^ mean(g v^)).
-// Bandwidth bound: a row lives in the registers of its threads (one wave up to 2048 elements, else one workgroup), so
-// that forward reads x and block once and backward gy, gn, y and block once.  Sums and statistics are float32; y is
+// Bandwidth bound: a row lives in the registers of its threads (16 lanes to 1024 threads, one 16-byte chunk each as long as
+// that is enough), so that forward reads x and block once and backward gy, gn, y and block once.  Workgroups stay and take
+// row after row: the next row's chunks are under way while the sums of this one cross the waves, and the weights' chunks
+// are held throughout.  Sums and statistics are float32; y is
 // normalised before it is rounded.  m and r of both norms are kept (16 bytes a row) so that backward uses the unrounded
 // rows' statistics.  The column sums of backward stay in registers over a workgroup's rows, go to a partial row per
 // workgroup and are added by a second launch in a fixed order (no atomics: results do not vary from run to run).
@@ -40,7 +42,7 @@ struct NormArgs {
     float scale, eps;
 };
 
-// Threads of one row: LANES of a wave (16, 32 or 64), or all of a workgroup of LANES = 256 or 512.
+// Threads of one row: LANES of a wave (16, 32 or 64) or LANES / 64 waves.
 template <int LANES> struct Row {
     static constexpr int THREADS = LANES < 256 ? 256 : LANES;
     static constexpr int ROWS = THREADS / LANES;                 // rows a workgroup works on at a time
@@ -51,30 +53,50 @@ template <int LANES> struct Row {
         for (int o = W / 2; o > 0; o /= 2) { a += __shfl_xor(a, o); b += __shfl_xor(b, o); }
         if constexpr (LANES > 64) {
             constexpr int WAVES = LANES / 64;
-            const int wave = threadIdx.x >> 6;
+            float* mine = scratch + threadIdx.x / LANES * (2 * WAVES);
             __syncthreads();                                      // the last sum's values have been read
-            if ((threadIdx.x & 63) == 0) { scratch[2 * wave] = a; scratch[2 * wave + 1] = b; }
+            if ((threadIdx.x & 63) == 0) *(float2*)(mine + 2 * ((threadIdx.x % LANES) / 64)) = make_float2(a, b);
             __syncthreads();
             a = b = 0.0f;
 #pragma unroll
-            for (int w = 0; w < WAVES; ++w) { a += scratch[2 * w]; b += scratch[2 * w + 1]; }
+            for (int w = 0; w < WAVES; ++w) { a += mine[2 * w]; b += mine[2 * w + 1]; }
         }
     }
 };
 
 template <typename T, int NV> struct Regs { float v[NV][Chunk<T>::n]; };
+template <typename T, int NV> struct Packed { Vec<T> v[NV]; };           // as in memory
 
-template <typename T, int NV, int LANES>
-__device__ __forceinline__ void load_row(Regs<T, NV>& out, const T* row, int32_t d, int lane, bool live) {
+// Rows of whole chunks; rows whose last chunk is ragged; rows shorter than a chunk.  Loads never branch on the data's
+// end (a load whose result is merged with another path's is waited for on the spot): a chunk past the end repeats the
+// last whole one, and the ragged chunk is the last CE elements of the row, moved to its place when it is used.
+enum Width { WHOLE, RAGGED, TINY };
+
+template <typename T, int NV, int LANES, int WIDTH>
+__device__ __forceinline__ void load_row(Packed<T, NV>& out, const T* row, int32_t d, int lane) {
     constexpr int CE = Chunk<T>::n;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = (i * LANES + lane) * CE;
-        Vec<T> t;
-        if (live && c < d) t = load_part(row + c, (int64_t)d - c);
-#pragma unroll
-        for (int e = 0; e < CE; ++e) out.v[i][e] = live && c < d ? to_f32(t.e[e]) : 0.0f;
+        if constexpr (WIDTH == TINY) out.v[i] = load_part(row, c == 0 ? d : 0);
+        else out.v[i] = load_chunk(row + (c < d - CE ? c : d - CE));
     }
+}
+// the values of chunk i in float32, zero from d on
+template <typename T, int NV, int LANES, int WIDTH>
+__device__ __forceinline__ void unpack(float (&out)[Chunk<T>::n], const Packed<T, NV>& in, int i, int32_t d, int lane, bool live = true) {
+    constexpr int CE = Chunk<T>::n;
+    const int c = (i * LANES + lane) * CE;
+    Vec<T> v = in.v[i];
+    if constexpr (WIDTH == RAGGED) {              // the first element wanted is number c - (d - CE) of those loaded
+        const int by = c > d - CE ? c - (d - CE) : 0;
+#pragma unroll
+        for (int step = 1; step < CE; step *= 2)
+#pragma unroll
+            for (int e = 0; e < CE; ++e) v.e[e] = (by & step) && e + step < CE ? v.e[e + step] : v.e[e];
+    }
+#pragma unroll
+    for (int e = 0; e < CE; ++e) out[e] = live && c + e < d ? to_f32(v.e[e]) : 0.0f;
 }
 template <typename T, int NV, int LANES>
 __device__ __forceinline__ void store_row(T* row, const Regs<T, NV>& in, int32_t d, int lane, bool live) {
@@ -114,31 +136,60 @@ __device__ __forceinline__ void row_stats(const Regs<T, NV>& v, int32_t d, int l
     r = 1.0f / sqrtf(q / (float)d + eps);
 }
 
-template <typename T, int NV, int LANES>
+template <typename T, int NV, int LANES, int WIDTH>
 __global__ __launch_bounds__(Row<LANES>::THREADS) void residual_norm_kernel(const NormArgs a) {
     using R = Row<LANES>;
+    using P = Packed<T, NV>;
     __shared__ float scratch[32];
     const int lane = threadIdx.x % LANES, slot = threadIdx.x / LANES;
     const int32_t d = a.d;
-    for (int64_t r0 = (int64_t)blockIdx.x * R::ROWS; r0 < a.rows; r0 += (int64_t)gridDim.x * R::ROWS) {
+    P wpost, wpre, gate, nb, nx;
+    load_row<T, NV, LANES, WIDTH>(wpost, (const T*)a.w_post, d, lane);
+    load_row<T, NV, LANES, WIDTH>(wpre, (const T*)a.w_pre, d, lane);
+    if (a.gate_kind == CHANNEL_GATE) load_row<T, NV, LANES, WIDTH>(gate, (const T*)a.gate, d, lane);
+    auto fetch = [&](int64_t r0, P& b, P& x) {
+        const int64_t r = r0 + slot < a.rows ? r0 + slot : a.rows - 1;
+        load_row<T, NV, LANES, WIDTH>(b, (const T*)a.block + r * a.ldb, d, lane);
+        load_row<T, NV, LANES, WIDTH>(x, (const T*)a.x + r * a.ldx, d, lane);
+    };
+    const int64_t turn = (int64_t)gridDim.x * R::ROWS;
+    int64_t r0 = (int64_t)blockIdx.x * R::ROWS;
+    fetch(r0, nb, nx);
+    for (; r0 < a.rows; r0 += turn) {
         const bool live = r0 + slot < a.rows;
         const int64_t r = live ? r0 + slot : a.rows - 1;
-        Regs<T, NV> b, y, w;
-        load_row<T, NV, LANES>(b, (const T*)a.block + r * a.ldb, d, lane, live);
-        load_row<T, NV, LANES>(y, (const T*)a.x + r * a.ldx, d, lane, live);
+        const P x = nx;
+        Regs<T, NV> b, y;
+        float w[Chunk<T>::n];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) unpack<T, NV, LANES, WIDTH>(b.v[i], nb, i, d, lane);
+        if (r0 + turn < a.rows) fetch(r0 + turn, nb, nx);
         float mb, rb, my, ry;
         row_stats<T, NV, LANES>(b, d, lane, a.layer, a.eps, scratch, mb, rb);
-        load_row<T, NV, LANES>(w, (const T*)a.w_post, d, lane, true);
-        FOR_ROW(i, e) b.v[i][e] = (b.v[i][e] - mb) * rb * w.v[i][e];
-        if (a.gate_kind != NO_GATE) {
-            load_row<T, NV, LANES>(w, (const T*)a.gate + (a.gate_kind == ROW_GATE ? r * a.ldg : 0), d, lane, true);
-            FOR_ROW(i, e) b.v[i][e] *= w.v[i][e];
+        if (a.gate_kind == ROW_GATE) load_row<T, NV, LANES, WIDTH>(gate, (const T*)a.gate + r * a.ldg, d, lane);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            constexpr int CE = Chunk<T>::n;
+            unpack<T, NV, LANES, WIDTH>(w, wpost, i, d, lane);
+#pragma unroll
+            for (int e = 0; e < CE; ++e) b.v[i][e] = (b.v[i][e] - mb) * rb * w[e];
+            if (a.gate_kind != NO_GATE) {
+                unpack<T, NV, LANES, WIDTH>(w, gate, i, d, lane);
+#pragma unroll
+                for (int e = 0; e < CE; ++e) b.v[i][e] *= w[e];
+            }
+            unpack<T, NV, LANES, WIDTH>(y.v[i], x, i, d, lane);
+#pragma unroll
+            for (int e = 0; e < CE; ++e) y.v[i][e] = fmaf(a.scale, y.v[i][e], b.v[i][e]);
         }
-        FOR_ROW(i, e) y.v[i][e] = fmaf(a.scale, y.v[i][e], b.v[i][e]);
         store_row<T, NV, LANES>((T*)a.y + r * d, y, d, lane, live);
         row_stats<T, NV, LANES>(y, d, lane, a.layer, a.eps, scratch, my, ry);
-        load_row<T, NV, LANES>(w, (const T*)a.w_pre, d, lane, true);
-        FOR_ROW(i, e) y.v[i][e] = (y.v[i][e] - my) * ry * w.v[i][e];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            unpack<T, NV, LANES, WIDTH>(w, wpre, i, d, lane);
+#pragma unroll
+            for (int e = 0; e < Chunk<T>::n; ++e) y.v[i][e] = (y.v[i][e] - my) * ry * w[e];
+        }
         store_row<T, NV, LANES>((T*)a.n + r * d, y, d, lane, live);
         if (a.stats && live && lane == 0) *(float4*)(a.stats + 4 * r) = make_float4(mb, rb, my, ry);
     }
@@ -155,49 +206,84 @@ __device__ __forceinline__ void norm_back(Regs<T, NV>& g, const Regs<T, NV>& h, 
     FOR_ROW(i, e) g.v[i][e] = r * (g.v[i][e] - s - h.v[i][e] * p);
 }
 
-template <typename T, int NV, int LANES>
+template <typename T, int NV, int LANES, int WIDTH>
 __global__ __launch_bounds__(Row<LANES>::THREADS) void residual_norm_backward_kernel(const NormArgs a) {
     using R = Row<LANES>;
     constexpr int CE = Chunk<T>::n;
     __shared__ float scratch[32];
     __shared__ float columns[R::ROWS > 1 ? R::THREADS * NV * CE : 1];       // one sum at a time
+    using P = Packed<T, NV>;
     const int lane = threadIdx.x % LANES, slot = threadIdx.x / LANES;
     const int32_t d = a.d;
     Regs<T, NV> spost = {}, spre = {}, sgate = {};
-    for (int64_t r0 = (int64_t)blockIdx.x * R::ROWS; r0 < a.rows; r0 += (int64_t)gridDim.x * R::ROWS) {
+    P wpost, wpre, gate, ny, ngn, ngy, nb;
+    float4 nst;
+    load_row<T, NV, LANES, WIDTH>(wpost, (const T*)a.w_post, d, lane);
+    load_row<T, NV, LANES, WIDTH>(wpre, (const T*)a.w_pre, d, lane);
+    if (a.gate_kind == CHANNEL_GATE) load_row<T, NV, LANES, WIDTH>(gate, (const T*)a.gate, d, lane);
+    auto fetch = [&](int64_t r0) {
+        const int64_t r = r0 + slot < a.rows ? r0 + slot : a.rows - 1;
+        nst = *(const float4*)(a.stats + 4 * r);
+        load_row<T, NV, LANES, WIDTH>(ny, (const T*)a.y + r * d, d, lane);
+        load_row<T, NV, LANES, WIDTH>(nb, (const T*)a.block + r * a.ldb, d, lane);
+        if (a.gn) load_row<T, NV, LANES, WIDTH>(ngn, (const T*)a.gn + r * a.ldgn, d, lane);
+        if (a.gy) load_row<T, NV, LANES, WIDTH>(ngy, (const T*)a.gy + r * a.ldgy, d, lane);
+    };
+    const int64_t turn = (int64_t)gridDim.x * R::ROWS;
+    int64_t r0 = (int64_t)blockIdx.x * R::ROWS;
+    fetch(r0);
+    for (; r0 < a.rows; r0 += turn) {
         const bool live = r0 + slot < a.rows;
         const int64_t r = live ? r0 + slot : a.rows - 1;
-        const float4 st = *(const float4*)(a.stats + 4 * r);
-        Regs<T, NV> h, t, w, o;
-        load_row<T, NV, LANES>(h, (const T*)a.y + r * d, d, lane, live);
-        load_row<T, NV, LANES>(t, (const T*)a.gn + r * a.ldgn, d, lane, live && a.gn);
-        load_row<T, NV, LANES>(w, (const T*)a.w_pre, d, lane, true);
-        FOR_ROW(i, e) {
-            h.v[i][e] = live && (i * LANES + lane) * CE + e < d ? (h.v[i][e] - st.z) * st.w : 0.0f;
-            spre.v[i][e] = fmaf(t.v[i][e], h.v[i][e], spre.v[i][e]);
-            t.v[i][e] *= w.v[i][e];
-        }
-        norm_back<T, NV, LANES>(t, h, d, a.layer, st.w, scratch);
-        load_row<T, NV, LANES>(w, (const T*)a.gy + r * a.ldgy, d, lane, live && a.gy);
-        FOR_ROW(i, e) { t.v[i][e] += w.v[i][e]; w.v[i][e] = a.scale * t.v[i][e]; }
-        store_row<T, NV, LANES>((T*)a.dx + r * d, w, d, lane, live);
-        load_row<T, NV, LANES>(h, (const T*)a.block + r * a.ldb, d, lane, live);
-        FOR_ROW(i, e) h.v[i][e] = live && (i * LANES + lane) * CE + e < d ? (h.v[i][e] - st.x) * st.y : 0.0f;
-        load_row<T, NV, LANES>(w, (const T*)a.w_post, d, lane, true);
-        if (a.gate_kind != NO_GATE) {
-            load_row<T, NV, LANES>(o, (const T*)a.gate + (a.gate_kind == ROW_GATE ? r * a.ldg : 0), d, lane, live);
-            Regs<T, NV> dg;
-            FOR_ROW(i, e) {
-                dg.v[i][e] = t.v[i][e] * h.v[i][e] * w.v[i][e];
-                sgate.v[i][e] += dg.v[i][e];
-                t.v[i][e] *= o.v[i][e];
+        const float4 st = nst;
+        const P gy = ngy, block = nb;
+        auto there = [&](int i, int e) { return live && (i * LANES + lane) * CE + e < d; };
+        Regs<T, NV> h, t;
+        float w[CE], g[CE];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            unpack<T, NV, LANES, WIDTH>(h.v[i], ny, i, d, lane);
+            unpack<T, NV, LANES, WIDTH>(g, ngn, i, d, lane, live && a.gn);
+            unpack<T, NV, LANES, WIDTH>(w, wpre, i, d, lane);
+#pragma unroll
+            for (int e = 0; e < CE; ++e) {
+                h.v[i][e] = there(i, e) ? (h.v[i][e] - st.z) * st.w : 0.0f;
+                spre.v[i][e] = fmaf(g[e], h.v[i][e], spre.v[i][e]);
+                t.v[i][e] = g[e] * w[e];
             }
-            if (a.gate_kind == ROW_GATE) store_row<T, NV, LANES>((T*)a.dgate_rows + r * d, dg, d, lane, live);
         }
-        FOR_ROW(i, e) {
-            if (live) spost.v[i][e] = fmaf(t.v[i][e], h.v[i][e], spost.v[i][e]);
-            t.v[i][e] *= w.v[i][e];
+        if (a.gate_kind == ROW_GATE) load_row<T, NV, LANES, WIDTH>(gate, (const T*)a.gate + r * a.ldg, d, lane);
+        if (r0 + turn < a.rows) fetch(r0 + turn);
+        norm_back<T, NV, LANES>(t, h, d, a.layer, st.w, scratch);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            unpack<T, NV, LANES, WIDTH>(g, gy, i, d, lane, live && a.gy);
+#pragma unroll
+            for (int e = 0; e < CE; ++e) {
+                t.v[i][e] += g[e];
+                h.v[i][e] = a.scale * t.v[i][e];
+            }
         }
+        store_row<T, NV, LANES>((T*)a.dx + r * d, h, d, lane, live);
+        Regs<T, NV> dg;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            unpack<T, NV, LANES, WIDTH>(h.v[i], block, i, d, lane);
+            unpack<T, NV, LANES, WIDTH>(w, wpost, i, d, lane);
+            if (a.gate_kind != NO_GATE) unpack<T, NV, LANES, WIDTH>(g, gate, i, d, lane);
+#pragma unroll
+            for (int e = 0; e < CE; ++e) {
+                h.v[i][e] = there(i, e) ? (h.v[i][e] - st.x) * st.y : 0.0f;
+                if (a.gate_kind != NO_GATE) {
+                    dg.v[i][e] = t.v[i][e] * h.v[i][e] * w[e];
+                    if (live) sgate.v[i][e] += dg.v[i][e];
+                    t.v[i][e] *= g[e];
+                }
+                if (live) spost.v[i][e] = fmaf(t.v[i][e], h.v[i][e], spost.v[i][e]);
+                t.v[i][e] *= w[e];
+            }
+        }
+        if (a.gate_kind == ROW_GATE) store_row<T, NV, LANES>((T*)a.dgate_rows + r * d, dg, d, lane, live);
         norm_back<T, NV, LANES>(t, h, d, a.layer, st.y, scratch);
         store_row<T, NV, LANES>((T*)a.dblock + r * d, t, d, lane, live);
     }
@@ -223,7 +309,7 @@ __global__ __launch_bounds__(Row<LANES>::THREADS) void residual_norm_backward_ke
     if (a.gate_kind == CHANNEL_GATE) put(2, sgate);
 }
 
-// dw_post, dw_pre, dgate: the partial rows added in order.  64 columns per workgroup, its 16 waves... rows split 16 ways.
+// dw_post, dw_pre, dgate: the partial rows added in a fixed order.  64 columns per workgroup, every 16th row per wave.
 template <typename T>
 __global__ __launch_bounds__(1024) void sum_columns_kernel(const float* __restrict__ partial, int blocks, int32_t d, T* __restrict__ o0, T* __restrict__ o1, T* __restrict__ o2) {
     __shared__ float part[16][64];
@@ -231,6 +317,7 @@ __global__ __launch_bounds__(1024) void sum_columns_kernel(const float* __restri
     const int which = blockIdx.y, c = blockIdx.x * 64 + lane;
     float s = 0.0f;
     if (c < d)
+#pragma unroll 8
         for (int b = wave; b < blocks; b += 16) s += partial[((int64_t)b * 3 + which) * d + c];
     part[wave][lane] = s;
     __syncthreads();
@@ -243,21 +330,26 @@ __global__ __launch_bounds__(1024) void sum_columns_kernel(const float* __restri
     }
 }
 
-constexpr int MAX_BLOCKS = 512;              // partial rows of backward
+// partial rows of backward: two workgroups of 512 threads or four of 256 on each of 256 CUs
+constexpr int max_blocks(int32_t d) { return d <= 1024 ? 1024 : 512; }
 
-// Threads per row and chunks per thread by width: FN<T, NV, LANES>.  Up to 32 elements per thread.
+// Threads per row and chunks per thread by width
 template <typename T, class F> hipError_t by_width(int32_t d, F&& f) {
     const int chunks = (d + Chunk<T>::n - 1) / Chunk<T>::n;
-#define MARL_ROW(NV, LANES) return f(std::integral_constant<int, NV>{}, std::integral_constant<int, LANES>{})
+    const bool whole = d % Chunk<T>::n == 0;
+#define MARL_ROW(NV, LANES)                                                                                                          \
+    return whole ? f(std::integral_constant<int, NV>{}, std::integral_constant<int, LANES>{}, std::integral_constant<int, WHOLE>{})  \
+                 : f(std::integral_constant<int, NV>{}, std::integral_constant<int, LANES>{}, std::integral_constant<int, RAGGED>{})
+    if (d < Chunk<T>::n) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{}, std::integral_constant<int, TINY>{});
     if (chunks <= 16) MARL_ROW(1, 16);
     if (chunks <= 32) MARL_ROW(1, 32);
     if (chunks <= 64) MARL_ROW(1, 64);
-    if (chunks <= 128) MARL_ROW(2, 64);
-    if (chunks <= 256) MARL_ROW(4, 64);
-    if (chunks <= 512) MARL_ROW(2, 256);
-    if (chunks <= 1024) MARL_ROW(4, 256);
-    if (chunks <= 2048) MARL_ROW(4, 512);
-    if constexpr (Chunk<T>::n == 4) { if (chunks <= 4096) MARL_ROW(8, 512); }
+    if (chunks <= 128) MARL_ROW(1, 128);
+    if (chunks <= 256) MARL_ROW(1, 256);
+    if (chunks <= 512) MARL_ROW(1, 512);
+    if (chunks <= 1024) MARL_ROW(2, 512);
+    if (chunks <= 2048) MARL_ROW(2, 1024);
+    if constexpr (Chunk<T>::n == 4) { if (chunks <= 4096) MARL_ROW(4, 1024); }
 #undef MARL_ROW
     return hipErrorInvalidValue;
 }
@@ -269,23 +361,24 @@ int done(hipError_t err) {
 }
 
 template <typename T> int forward(const NormArgs& a, hipStream_t stream) {
-    return done(by_width<T>(a.d, [&](auto nv, auto lanes) {
-        constexpr int NV = decltype(nv)::value, LANES = decltype(lanes)::value;
+    return done(by_width<T>(a.d, [&](auto nv, auto lanes, auto width) {
+        constexpr int NV = decltype(nv)::value, LANES = decltype(lanes)::value, WIDTH = decltype(width)::value;
         using R = Row<LANES>;
-        const int64_t blocks = (a.rows + R::ROWS - 1) / R::ROWS;
-        hipLaunchKernelGGL((residual_norm_kernel<T, NV, LANES>), dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(R::THREADS), 0, stream, a);
+        const int64_t blocks = (a.rows + R::ROWS - 1) / R::ROWS, most = 256 * (2048 / R::THREADS);      // as many as the chip holds
+        hipLaunchKernelGGL((residual_norm_kernel<T, NV, LANES, WIDTH>), dim3((unsigned)(blocks < most ? blocks : most)), dim3(R::THREADS), 0, stream, a);
         return hipGetLastError();
     }));
 }
 
 template <typename T> int backward(const NormArgs& a, void* dw_post, void* dw_pre, void* dgate, hipStream_t stream) {
     int blocks = 0;
-    hipError_t err = by_width<T>(a.d, [&](auto nv, auto lanes) {
-        constexpr int NV = decltype(nv)::value, LANES = decltype(lanes)::value;
+    hipError_t err = by_width<T>(a.d, [&](auto nv, auto lanes, auto width) {
+        constexpr int NV = decltype(nv)::value, LANES = decltype(lanes)::value, WIDTH = decltype(width)::value;
         using R = Row<LANES>;
-        const int64_t want = (a.rows + R::ROWS - 1) / R::ROWS;
-        blocks = (int)(want < MAX_BLOCKS ? want : MAX_BLOCKS);
-        hipLaunchKernelGGL((residual_norm_backward_kernel<T, NV, LANES>), dim3(blocks), dim3(R::THREADS), 0, stream, a);
+        // four turns or more a workgroup, so that adding the partial rows stays cheap, but one for every CU if there are rows
+        const int64_t turns = (a.rows + R::ROWS - 1) / R::ROWS, want = turns / 4 > 256 ? turns / 4 : turns < 256 ? turns : 256;
+        blocks = (int)(want < max_blocks(a.d) ? want : max_blocks(a.d));
+        hipLaunchKernelGGL((residual_norm_backward_kernel<T, NV, LANES, WIDTH>), dim3(blocks), dim3(R::THREADS), 0, stream, a);
         return hipGetLastError();
     });
     if (err == hipSuccess) {
@@ -324,7 +417,7 @@ int marl_residual_norm(int32_t dtype, int32_t kind, int64_t rows, int32_t d, con
 }
 
 size_t marl_residual_norm_workspace_bytes(int32_t d) {
-    return d < 1 || d > MARL_MAX_NORM_WIDTH ? 0 : (size_t)MAX_BLOCKS * 3 * d * sizeof(float);
+    return d < 1 || d > MARL_MAX_NORM_WIDTH ? 0 : (size_t)max_blocks(d) * 3 * d * sizeof(float);
 }
 
 int marl_residual_norm_backward(int32_t dtype, int32_t kind, int64_t rows, int32_t d, const void* y, const void* block, int64_t ld_block,
