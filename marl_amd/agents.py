@@ -8,12 +8,16 @@ values never leave the GPU, E environments are acted on at once, the rollout
 lives in `DeviceRolloutBuffer`, GAE runs in libmarl_env.so, and with more than
 one rank the gradients of both networks travel in ONE flat all-reduce per
 optimiser step (RCCL over xGMI; 145 KB, latency bound).
+
+Beyond the reference, `trunk="gated"` gives both networks a deeper trunk of residual blocks (GatedTrunk: gated_linear,
+residual_norm and keyed_dropout of torch.ops.marl_amd, GPU only), and `sampling=` draws the band with temperature, top-k,
+top-p and min-p (sample_logits).
 """
 from __future__ import annotations
 
 import ctypes as C
 from pathlib import Path
-from typing import Dict, List, Optional, Tuple
+from typing import Dict, List, NamedTuple, Optional, Tuple
 
 import numpy as np
 import torch
@@ -68,16 +72,75 @@ class TallLinear(nn.Linear):
         return super().forward(x)
 
 
+class BandSampling(NamedTuple):
+    """How a band is drawn from its logits: temperature (0: the largest), then the top_k largest (0: all), the shortest
+    prefix of them that holds top_p of their mass, those with at least min_p of the largest one's probability."""
+    temperature: float = 1.0
+    top_k: int = 0
+    top_p: float = 1.0
+    min_p: float = 0.0
+
+
+class GatedBlock(nn.Module):
+    """x, n -> x', n':  x' = x + gate * N(down(dropout(act(n Wg^T) * (n Wu^T)))),  n' = N(x')."""
+
+    def __init__(self, dim, inner, dropout=0.0, act="silu"):
+        super().__init__()
+        self.dropout, self.act = float(dropout), act
+        self.w_gate, self.w_up = nn.Parameter(torch.empty(inner, dim)), nn.Parameter(torch.empty(inner, dim))
+        self.down = TallLinear(inner, dim)
+        self.post, self.pre = nn.Parameter(torch.ones(dim)), nn.Parameter(torch.ones(dim))
+        self.gate = nn.Parameter(torch.full((dim,), 0.5))
+        for w in (self.w_gate, self.w_up):
+            nn.init.orthogonal_(w, gain=np.sqrt(2))
+
+    def forward(self, x, n, seed=0, keys=None):
+        ops = torch.ops.marl_amd
+        h = ops.gated_linear(n, self.w_gate, self.w_up, self.act)
+        if keys is not None and self.dropout > 0.0 and self.training:
+            h = ops.keyed_dropout(h, self.dropout, seed, keys)
+        return ops.residual_norm(x, self.down(h), self.post, self.pre, self.gate, 1.0, 1e-5, "layer")
+
+
+class GatedTrunk(nn.Module):
+    """obs -> hidden -> `blocks` residual blocks (GatedBlock), the features normalised.  Runs on the GPU only.
+
+    Dropout is consistent: the mask of a row is a function of (dropout_seed, block, row key), so the update of a PPO step,
+    which meets the rollout's rows shuffled, works with the masks the rows were acted with; with masks drawn anew the
+    probability ratio would compare two different networks.  Rows without keys pass without dropout."""
+
+    def __init__(self, obs_dim=5, hidden_dim=128, blocks=2, inner=4, dropout=0.0, dropout_seed=0):
+        super().__init__()
+        from . import ops  # noqa: F401  registers torch.ops.marl_amd
+        self.dropout, self.dropout_seed = float(dropout), int(dropout_seed)
+        self.embed, self.norm = TallLinear(obs_dim, hidden_dim), nn.LayerNorm(hidden_dim)
+        self.blocks = nn.ModuleList(GatedBlock(hidden_dim, inner * hidden_dim, dropout) for _ in range(blocks))
+
+    def forward(self, obs, keys=None):
+        x = self.embed(obs)
+        n = self.norm(x)
+        for i, block in enumerate(self.blocks):
+            x, n = block(x, n, self.dropout_seed + i, keys)
+        return n
+
+
 class Actor(nn.Module):
     """agents/actor.py:56-247: 5 -> hidden -> hidden (LayerNorm + ReLU) trunk, heads for
-    velocity mean (2), clamped log-std (2) and band logits (num_bands)."""
+    velocity mean (2), clamped log-std (2) and band logits (num_bands).  trunk="gated": a GatedTrunk instead."""
 
-    def __init__(self, obs_dim=5, hidden_dim=128, v_max=5.0, num_bands=4, log_std_min=-2.0, log_std_max=2.0):
+    def __init__(self, obs_dim=5, hidden_dim=128, v_max=5.0, num_bands=4, log_std_min=-2.0, log_std_max=2.0, trunk="mlp",
+                 trunk_blocks=2, trunk_dropout=0.0, dropout_seed=0):
         super().__init__()
         self.obs_dim, self.hidden_dim, self.v_max, self.num_bands = obs_dim, hidden_dim, v_max, num_bands
         self.log_std_min, self.log_std_max = log_std_min, log_std_max
-        self.trunk = nn.Sequential(TallLinear(obs_dim, hidden_dim), nn.LayerNorm(hidden_dim), nn.ReLU(),
-                                   TallLinear(hidden_dim, hidden_dim), nn.LayerNorm(hidden_dim), nn.ReLU())
+        if trunk not in ("mlp", "gated"):
+            raise ValueError(f"trunk must be mlp or gated, not {trunk!r}")
+        self.gated = trunk == "gated"
+        if self.gated:
+            self.trunk = GatedTrunk(obs_dim, hidden_dim, trunk_blocks, dropout=trunk_dropout, dropout_seed=dropout_seed)
+        else:
+            self.trunk = nn.Sequential(TallLinear(obs_dim, hidden_dim), nn.LayerNorm(hidden_dim), nn.ReLU(),
+                                       TallLinear(hidden_dim, hidden_dim), nn.LayerNorm(hidden_dim), nn.ReLU())
         self.mu_head = TallLinear(hidden_dim, 2)
         self.log_std_head = TallLinear(hidden_dim, 2)
         self.band_head = TallLinear(hidden_dim, num_bands)
@@ -90,13 +153,16 @@ class Actor(nn.Module):
         nn.init.constant_(self.log_std_head.bias, -0.5)
         nn.init.orthogonal_(self.band_head.weight, gain=0.01)
 
-    def forward(self, obs):
-        f = self.trunk(obs)
+    def forward(self, obs, keys=None):
+        f = self.trunk(obs, keys) if self.gated else self.trunk(obs)
         return self.mu_head(f), torch.clamp(self.log_std_head(f), self.log_std_min, self.log_std_max), self.band_head(f)
 
-    def sample(self, obs, deterministic=False, generator: Optional[torch.Generator] = None):
-        """actor.py:146-202.  obs [..., obs_dim] -> actions [..., 3], log_prob [...], entropy [...]."""
-        mu, log_std, logits = self.forward(obs)
+    def sample(self, obs, deterministic=False, generator: Optional[torch.Generator] = None, keys=None,
+               sampling: Optional[BandSampling] = None):
+        """actor.py:146-202.  obs [..., obs_dim] -> actions [..., 3], log_prob [...], entropy [...].  keys [...] (int64): the
+        rows' dropout keys.  sampling (GPU only): the band is drawn that way; its log-probability is the one among the bands
+        that were left, the entropy stays that of the whole distribution."""
+        mu, log_std, logits = self.forward(obs, keys)
         std = torch.exp(log_std)
         # validate_args=False: the argument checks read a flag back to the host at every call
         vdist, bdist = Normal(mu, std, validate_args=False), Categorical(logits=logits, validate_args=False)
@@ -109,14 +175,19 @@ class Actor(nn.Module):
                 velocity = mu + std * torch.randn(mu.shape, device=mu.device, dtype=mu.dtype, generator=generator)
                 band = torch.multinomial(bdist.probs.reshape(-1, self.num_bands), 1,
                                          generator=generator).reshape(logits.shape[:-1])
-        log_prob = vdist.log_prob(velocity).sum(dim=-1) + bdist.log_prob(band)
+        band_log_prob = None
+        if sampling is not None and not deterministic:
+            from . import ops  # noqa: F401  registers torch.ops.marl_amd
+            u = torch.rand(logits.shape[:-1], device=logits.device, generator=generator)
+            band, band_log_prob = torch.ops.marl_amd.sample_logits(logits, u, *sampling)
+        log_prob = vdist.log_prob(velocity).sum(dim=-1) + (bdist.log_prob(band) if band_log_prob is None else band_log_prob)
         entropy = vdist.entropy().sum(dim=-1) + bdist.entropy()
         actions = torch.cat([torch.clamp(velocity, -self.v_max, self.v_max), band.unsqueeze(-1).float()], dim=-1)
         return actions, log_prob, entropy
 
-    def evaluate_actions(self, obs, actions):
+    def evaluate_actions(self, obs, actions, keys=None):
         """actor.py:204-247."""
-        mu, log_std, logits = self.forward(obs)
+        mu, log_std, logits = self.forward(obs, keys)
         vdist = Normal(mu, torch.exp(log_std), validate_args=False)
         bdist = Categorical(logits=logits, validate_args=False)
         velocity = torch.clamp(actions[..., :2], -self.v_max * 2, self.v_max * 2)
@@ -127,13 +198,17 @@ class Actor(nn.Module):
 
 
 class Critic(nn.Module):
-    """agents/critic.py:53-134: 5 -> hidden -> hidden -> 1 on the mean-pooled observation."""
+    """agents/critic.py:53-134: 5 -> hidden -> hidden -> 1 on the mean-pooled observation.  trunk="gated": a GatedTrunk
+    (without dropout) before the last layer."""
 
-    def __init__(self, obs_dim=5, hidden_dim=128):
+    def __init__(self, obs_dim=5, hidden_dim=128, trunk="mlp", trunk_blocks=2):
         super().__init__()
         self.obs_dim, self.hidden_dim = obs_dim, hidden_dim
-        self.network = nn.Sequential(TallLinear(obs_dim, hidden_dim), nn.ReLU(), TallLinear(hidden_dim, hidden_dim),
-                                     nn.ReLU(), TallLinear(hidden_dim, 1))
+        if trunk == "gated":
+            self.network = nn.Sequential(GatedTrunk(obs_dim, hidden_dim, trunk_blocks), TallLinear(hidden_dim, 1))
+        else:
+            self.network = nn.Sequential(TallLinear(obs_dim, hidden_dim), nn.ReLU(), TallLinear(hidden_dim, hidden_dim),
+                                         nn.ReLU(), TallLinear(hidden_dim, 1))
         for m in self.modules():
             if isinstance(m, nn.Linear):
                 nn.init.orthogonal_(m.weight, gain=np.sqrt(2))
@@ -438,7 +513,8 @@ class PPOAgent:
     def __init__(self, obs_dim=5, hidden_dim=128, M=4, v_max=5.0, num_bands=4, log_std_min=-1.0, log_std_max=0.5,
                  gamma=0.99, gae_lambda=0.95, clip_eps=0.2, lr_actor=3e-4, lr_critic=1e-3, c1=0.5, c2=0.01,
                  max_grad_norm=0.5, rollout_length=2048, batch_size=256, n_epochs=10, device="auto", num_envs=1,
-                 seed: Optional[int] = None, fused_update: Optional[bool] = None):
+                 seed: Optional[int] = None, fused_update: Optional[bool] = None, trunk="mlp", trunk_blocks=2,
+                 trunk_dropout=0.0):
         self.obs_dim, self.hidden_dim, self.M, self.v_max, self.num_bands = obs_dim, hidden_dim, M, v_max, num_bands
         self.gamma, self.gae_lambda, self.clip_eps, self.c1, self.c2 = gamma, gae_lambda, clip_eps, c1, c2
         self.c2_initial, self.max_grad_norm = c2, max_grad_norm
@@ -448,8 +524,14 @@ class PPOAgent:
                                             else device)
         if seed is not None:
             torch.manual_seed(seed)
-        self.actor = Actor(obs_dim, hidden_dim, v_max, num_bands, log_std_min, log_std_max).to(self.device)
-        self.critic = Critic(obs_dim, hidden_dim).to(self.device)
+        self.trunk, self.trunk_blocks, self.trunk_dropout = trunk, int(trunk_blocks), float(trunk_dropout)
+        if trunk == "gated" and self.device.type != "cuda":
+            raise ValueError('trunk="gated" runs on the GPU only')
+        if not 0.0 <= self.trunk_dropout < 1.0 or (self.trunk_dropout > 0.0 and trunk != "gated"):
+            raise ValueError('trunk_dropout must be in [0, 1), and needs trunk="gated"')
+        self.actor = Actor(obs_dim, hidden_dim, v_max, num_bands, log_std_min, log_std_max, trunk, trunk_blocks, trunk_dropout,
+                           dropout_seed=0 if seed is None else int(seed) << 8).to(self.device)
+        self.critic = Critic(obs_dim, hidden_dim, trunk, trunk_blocks).to(self.device)
         if _dist_on():                       # every rank starts from rank 0's weights
             for p in list(self.actor.parameters()) + list(self.critic.parameters()):
                 torch.distributed.broadcast(p.data, src=0)
@@ -469,6 +551,13 @@ class PPOAgent:
         if self.device.type == "cuda":
             self.buffer = DeviceRolloutBuffer(rollout_length, num_envs, M, obs_dim, 3, gamma, gae_lambda, self.device)
         self.total_timesteps, self.total_updates = 0, 0
+        # Dropout keys: row (t, e, m) of a rollout is number (t E + e) M + m, counted on from rollout to rollout in device
+        # memory (a captured rollout replays with the keys of the current one) and apart for every rank.
+        self._row_base = None
+        if self.trunk_dropout > 0.0:
+            self._row_number = torch.arange(num_envs * M, device=self.device).view(num_envs, M)
+            self._row_base = torch.zeros((), dtype=torch.int64, device=self.device)
+            self._set_row_base()
         self.training_stats: Dict[str, List[float]] = {k: [] for k in
                                                        ("actor_loss", "critic_loss", "entropy", "clip_fraction",
                                                         "approx_kl")}
@@ -476,7 +565,8 @@ class PPOAgent:
         self._sample_gen = None
         # Acting through libmarl_env.so (marl_policy_act: both networks, the draws and the log-probabilities in
         # one launch) needs the weights as one packed buffer, refreshed whenever they change.
-        self.policy_kernel = self.device.type == "cuda" and hidden_dim in (64, 128) and num_bands == 4 and obs_dim == 5
+        self.policy_kernel = (self.device.type == "cuda" and hidden_dim in (64, 128) and num_bands == 4 and obs_dim == 5
+                              and trunk == "mlp")
         self._packed, self._packed_stale, self._act_calls = None, True, 0
         self.seed = 0 if seed is None else int(seed)
         # Minibatch step through libmarl_env.so (marl_ppo_rows: forward, losses and backward of every row in one
@@ -485,13 +575,26 @@ class PPOAgent:
         self._fz = None
 
     # -- acting (ppo_agent.py:193-225) ----------------------------------------
+    def _set_row_base(self):
+        rank = torch.distributed.get_rank() if _dist_on() else 0
+        self._row_base.fill_((rank << 48) + self.total_updates * self.rollout_length * self.E * self.M)
+
+    def _slot_keys(self, obs):
+        """Dropout keys of the rows acted on now, those of the buffer's current slot; None where no dropout applies."""
+        if self._row_base is None or not self.actor.training or tuple(obs.shape[:2]) != (self.E, self.M):
+            return None
+        return self._row_number + (self._row_base + self.buffer.pos * self.E * self.M)
+
     @torch.no_grad()
-    def get_action(self, obs, deterministic: bool = False):
+    def get_action(self, obs, deterministic: bool = False, sampling: Optional[BandSampling] = None):
+        """sampling: the band is drawn that way (BandSampling).  For acting outside of training: the update's ratio is to
+        the policy's whole distribution."""
         single = isinstance(obs, np.ndarray)
         o = torch.from_numpy(obs).float().to(self.device) if single else obs
         if o.dim() == 2:
             o = o.unsqueeze(0)
-        actions, log_probs, _ = self.actor.sample(o, deterministic, generator=self._sample_gen)
+        actions, log_probs, _ = self.actor.sample(o, deterministic, generator=self._sample_gen, keys=self._slot_keys(o),
+                                                  sampling=sampling)
         values = self.critic.forward_pooled(o.mean(dim=1)).squeeze(-1)
         if single:
             return actions[0].cpu().numpy(), log_probs[0].cpu().numpy(), float(values[0].item())
@@ -573,15 +676,17 @@ class PPOAgent:
         obs, actions, logp, adv, ret, _ = self.buffer.get_samples()
         stats = self.optimise(obs, actions, logp, adv, ret, permutations=permutations)
         self.total_updates += 1
+        if self._row_base is not None:
+            self._set_row_base()
         self.buffer.reset()
         for k, v in stats.items():
             self.training_stats[k].append(v)
         return stats
 
-    def _forward_backward(self, b_obs, b_act, b_old, b_adv, b_ret) -> torch.Tensor:
+    def _forward_backward(self, b_obs, b_act, b_old, b_adv, b_ret, keys=None) -> torch.Tensor:
         """Losses and gradients of one minibatch (ppo_agent.py:296-323, 328-329); returns [actor_loss,
         critic_loss, entropy, clip_fraction, approx_kl] as a float64 device tensor."""
-        log_probs, entropy = self.actor.evaluate_actions(b_obs, b_act)
+        log_probs, entropy = self.actor.evaluate_actions(b_obs, b_act, keys)
         values = self.critic.forward_pooled(b_obs).squeeze(-1)
         ratio = torch.exp(log_probs - b_old)
         surr1 = ratio * b_adv
@@ -751,10 +856,10 @@ class PPOAgent:
         self.actor_optimizer.step()
         self.critic_optimizer.step()
 
-    def _minibatch_step(self, b_obs, b_act, b_old, b_adv, b_ret) -> torch.Tensor:
+    def _minibatch_step(self, b_obs, b_act, b_old, b_adv, b_ret, keys=None) -> torch.Tensor:
         """One optimiser step of ppo_agent.py:296-345: gradients, their average over the ranks (one flat
         all-reduce), clip, Adam."""
-        out = self._forward_backward(b_obs, b_act, b_old, b_adv, b_ret)
+        out = self._forward_backward(b_obs, b_act, b_old, b_adv, b_ret, keys)
         self._sync.sync()
         self._apply_gradients()
         return out
@@ -801,7 +906,7 @@ class PPOAgent:
                     steps += 1
                     continue
                 batch = (obs[idx], actions[idx], old_log_probs[idx], advantages[idx], returns[idx])
-                out = self._minibatch_step(*batch)
+                out = self._minibatch_step(*batch, keys=None if self._row_base is None else idx + self._row_base)
                 acc += out
                 epoch_kl += out[4]
                 nb += 1
@@ -840,9 +945,11 @@ class PPOAgent:
         self.critic.train(training)
 
     def _config(self):
-        return {k: getattr(self, k) for k in ("obs_dim", "hidden_dim", "M", "v_max", "num_bands", "gamma",
-                                              "gae_lambda", "clip_eps", "c1", "c2", "max_grad_norm",
-                                              "rollout_length", "batch_size", "n_epochs")}
+        keys = ("obs_dim", "hidden_dim", "M", "v_max", "num_bands", "gamma", "gae_lambda", "clip_eps", "c1", "c2",
+                "max_grad_norm", "rollout_length", "batch_size", "n_epochs")
+        if self.trunk != "mlp":                  # the reference's constructor takes the others only
+            keys += ("trunk", "trunk_blocks", "trunk_dropout")
+        return {k: getattr(self, k) for k in keys}
 
     def save(self, path):
         """Same file name and keys as the reference checkpoint (ppo_agent.py:386-420); the statistics are
@@ -914,6 +1021,8 @@ class PPOAgent:
         if self._fz is not None:                       # the loaded moments into the flat vectors marl_ppo_apply steps
             self._flatten_optimizer_state()
         self._packed_stale = True
+        if self._row_base is not None:
+            self._set_row_base()
 
     def export_actor(self, path):
         """`actor_state_dict.pt` for the reference's deployment controller (deploy.py:139-188): the state

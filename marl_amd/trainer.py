@@ -214,10 +214,11 @@ class BatchedTrainer:
 
     # -- evaluation (training/trainer.py:326-385) -----------------------------------
     @torch.no_grad()
-    def evaluate(self, n_episodes: int = 5, deterministic: bool = False, num_envs: int = 256) -> Dict[str, float]:
+    def evaluate(self, n_episodes: int = 5, deterministic: bool = False, num_envs: int = 256, sampling=None) -> Dict[str, float]:
         """n_episodes episodes on each of `num_envs` fresh environments with the current policy: mean / std of
         the episode return and of the final lambda2 reduction, mean length, fraction of episodes in which the
-        graph was fragmented (lambda2 < 1e-10) at some step.  Does not touch the training environments."""
+        graph was fragmented (lambda2 < 1e-10) at some step.  Does not touch the training environments.
+        sampling (agents.BandSampling): how the bands are drawn."""
         cfg, agent = self.env_cfg, self.agent
         env = BatchedJammerEnv(num_envs, cfg, seed=self.seed + 7919 + self.total_rollouts, device=self.device,
                                auto_reset=False, env_offset=self.rank * num_envs)
@@ -232,12 +233,12 @@ class BatchedTrainer:
             ret = torch.zeros(num_envs, dtype=torch.float64, device=self.device)
             fragmented = torch.zeros(num_envs, dtype=torch.bool, device=self.device)
             for t in range(cfg.max_steps):
-                if agent.policy_kernel:
+                if agent.policy_kernel and sampling is None:
                     agent.act_kernel(obs, act, logp, None, tick=env.views["tick"], deterministic=deterministic,
                                      env_offset=env.env_offset)
                     a = act
                 else:
-                    a, _, _ = agent.get_action(obs, deterministic=deterministic)
+                    a, _, _ = agent.get_action(obs, deterministic=deterministic, sampling=sampling)
                 obs, reward, _, truncated, info = env.step(a)
                 ret += reward.double()
                 fragmented |= info["lambda2_current"] < 1e-10

@@ -99,3 +99,13 @@ def test_entry_points_check_their_arguments():
                 dict(m=-0.1), dict(m=1.1)):
         assert sl(**bad) == E, bad
     assert sl(V=(1 << 20) + 1, ld=1 << 21) == U
+
+
+def test_gated_trunk_is_refused_on_the_cpu_and_the_default_networks_are_unchanged():
+    from marl_amd.agents import Actor, Critic, PPOAgent
+    for bad in (dict(trunk="gated"), dict(trunk="conv"), dict(trunk_dropout=0.1), dict(trunk="gated", trunk_dropout=1.0)):
+        with pytest.raises(ValueError):
+            PPOAgent(device="cpu", **bad)
+    assert [k for k in Actor().state_dict()][:2] == ["trunk.0.weight", "trunk.0.bias"] and "network.4.bias" in Critic().state_dict()
+    agent = PPOAgent(device="cpu", seed=1)
+    assert set(agent._config()) & {"trunk", "trunk_blocks", "trunk_dropout"} == set()
