@@ -100,7 +100,8 @@ struct ProductArgs {
     int tiles_m, tiles_n;
 };
 
-// y, and f and p for backward, of `left` (at most a chunk) neighbouring columns from their a and b
+// y, and f and p for backward, of `left` (at most a chunk) neighbouring columns from their a and b; stored past the caches,
+// which hold the operands (T 32768, d 128, h 512, float32: 115 -> 103 us)
 template <typename T, int ACT> __device__ __forceinline__ void gate_out(const ProductArgs& args, int64_t at, const float* a, const float* b, int64_t left) {
     constexpr int CE = Chunk<T>::n;
     Vec<T> y, vf, vp;
@@ -112,10 +113,10 @@ template <typename T, int ACT> __device__ __forceinline__ void gate_out(const Pr
         vf.e[e] = from_f32<T>(f);
         vp.e[e] = from_f32<T>(b[e] * df);
     }
-    store_part((T*)args.out0 + at, y, left);
+    stream_part((T*)args.out0 + at, y, left);
     if (args.save_f) {
-        store_part((T*)args.save_f + at, vf, left);
-        store_part((T*)args.save_p + at, vp, left);
+        stream_part((T*)args.save_f + at, vf, left);
+        stream_part((T*)args.save_p + at, vp, left);
     }
 }
 

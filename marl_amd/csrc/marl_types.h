@@ -30,6 +30,8 @@ template <typename T> __device__ __forceinline__ Vec<T> load_chunk(const T* p) {
 template <typename T> __device__ __forceinline__ void store_chunk(T* p, const Vec<T>& v) {
     __builtin_memcpy(__builtin_assume_aligned(p, sizeof(T)), &v, 16);
 }
+typedef unsigned int uint4v __attribute__((ext_vector_type(4)));
+struct __attribute__((packed, aligned(2))) Unaligned { uint4v v; };
 // `left` elements remain from p on: whole chunks in one access, the last one element by element (the rest reads as zero)
 template <typename T> __device__ __forceinline__ Vec<T> load_part(const T* p, int64_t left) {
     constexpr int n = Chunk<T>::n;
@@ -42,6 +44,14 @@ template <typename T> __device__ __forceinline__ Vec<T> load_part(const T* p, in
 template <typename T> __device__ __forceinline__ void store_part(T* p, const Vec<T>& v, int64_t left) {
     constexpr int n = Chunk<T>::n;
     if (left >= n) { store_chunk(p, v); return; }
+#pragma unroll
+    for (int i = 0; i < n; ++i) if (i < left) p[i] = v.e[i];
+}
+
+// the same for results that nothing reads soon: past the caches
+template <typename T> __device__ __forceinline__ void stream_part(T* p, const Vec<T>& v, int64_t left) {
+    constexpr int n = Chunk<T>::n;
+    if (left >= n) { __builtin_nontemporal_store(__builtin_bit_cast(uint4v, v), &((Unaligned*)p)->v); return; }
 #pragma unroll
     for (int i = 0; i < n; ++i) if (i < left) p[i] = v.e[i];
 }
