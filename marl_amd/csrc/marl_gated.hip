@@ -133,13 +133,13 @@ template <typename T> __device__ __forceinline__ int tile_k_across(int kr, int c
 
 typedef __attribute__((address_space(3))) char lds_char;
 
-// 16 bytes per lane from `src` to LDS at `dst` (the same for the whole wave) + 16 lane.  In assembly because the compiler
-// makes every LDS read behind the builtin wait for all of these loads; here wait_loads() counts them.  The statement has no
-// output registers, and the wait on M0 is inside it.
-__device__ __forceinline__ void load_to_lds(const void* src, char* dst) {
-    const int at = __builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(lds_char*)dst);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(src) : "memory", "m0");
+// 16 bytes per lane from `base` + `off` (bytes) to LDS at `dst` (the same for the whole wave, as `base`) + 16 lane.  In
+// assembly because the compiler makes every LDS read behind the builtin wait for all of these loads; here wait_loads()
+// counts them.  The statement has no output registers, and its wait on M0 is inside it.
+__device__ __forceinline__ void load_to_lds(const char* base, uint32_t off, int dst) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(off), "s"(base) : "memory", "m0");
 }
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // One operand's tile: ROWS rows (m or n) by ROW_BYTES of k.  ACROSS: k runs across the rows of memory.
 template <typename T, int MODE, bool IS_B, int ROWS, int THREADS>
@@ -173,36 +173,55 @@ struct Tile {
             return (const T*)o.p0 + rr * o.ld0 + (MODE == DX && second ? a.half : 0);
         }
     }
-    // The thread's chunks at k = 0, found once: a stage then adds one offset to all of them.  DX's B: of both weights.
-    struct Pointers {
-        const T* at[PER];
-        const T* at2[MODE == DX && IS_B ? PER : 1];
+    // Where the thread's chunks of a stage come from: bytes from a base that is the same for the wave and moves on by
+    // `step` bytes a stage.  FWD's B has two weights; the 16 rows of one load of a wave are all of one of them.
+    static constexpr int BASES = MODE == FWD && IS_B ? PER : 1;
+    struct Source {
+        const char* base[BASES];
+        uint32_t off[PER];
+        int64_t step;
     };
-    static __device__ __forceinline__ void pointers(const ProductArgs& a, int64_t row0, int64_t rows, Pointers& p) {
+    static __device__ __forceinline__ void source(const ProductArgs& a, int64_t row0, int64_t rows, Source& src) {
+        const Operand& o = IS_B ? a.B : a.A;
+        src.step = (ACROSS ? BK * o.ld0 : BK) * (int64_t)sizeof(T);
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             int r, e;
             place(i * THREADS + (int)threadIdx.x, r, e);
-            // columns beyond the edge repeat the last chunk
-            const int64_t col = !ACROSS ? e : row0 + e < rows ? row0 + e : (rows - 1) / CE * CE;
-            p.at[i] = row_ptr(a, row0, rows, 0, r, false) + col;
-            if constexpr (MODE == DX && IS_B) p.at2[i] = row_ptr(a, row0, rows, 0, r, true) + col;
+            int64_t at;
+            if constexpr (ACROSS) {                // columns beyond the edge repeat the last chunk
+                const int64_t col = row0 + e < rows ? row0 + e : (rows - 1) / CE * CE;
+                at = r * o.ld0 + col - row0;
+                src.base[0] = (const char*)((const T*)o.p0 + row0);
+            } else if constexpr (MODE == FWD && IS_B) {
+                const bool up = uniform(r & 32) != 0;
+                const int64_t ld = up ? o.ld1 : o.ld0, row = row0 / 2 + (r / 64) * 32 + (r & 31), rr = row < rows ? row : rows - 1;
+                at = (rr - row0 / 2) * ld + e;
+                src.base[i] = (const char*)((const T*)(up ? o.p1 : o.p0) + row0 / 2 * ld);
+            } else {
+                const int64_t row = row0 + r, rr = row < rows ? row : rows - 1;
+                at = (rr - row0) * o.ld0 + e;
+                src.base[0] = (const char*)((const T*)o.p0 + row0 * o.ld0);
+            }
+            src.off[i] = (uint32_t)(at * (int64_t)sizeof(T));
         }
     }
-    static __device__ __forceinline__ int64_t offset(const ProductArgs& a, int64_t k0, bool second) {
+    // to whole stage n of the first pass over k, or of the second (DX: db against the second weight)
+    static __device__ __forceinline__ void seek(const ProductArgs& a, int64_t row0, int n, bool second, Source& src) {
         const Operand& o = IS_B ? a.B : a.A;
-        if constexpr (ACROSS) return k0 * (MODE == DX && second ? o.ld1 : o.ld0);
-        return k0 + (MODE == DX && second ? a.half : 0);
-    }
-    // whole stage from k0 on, direct global -> LDS
-    static __device__ __forceinline__ void load_direct(const ProductArgs& a, const Pointers& p, int64_t k0, bool second, char* lds) {
-        const int64_t step = offset(a, k0, second);
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const T* src = p.at[i];
-            if constexpr (MODE == DX && IS_B) src = second ? p.at2[i] : src;
-            load_to_lds(src + step, lds + (i * THREADS + (threadIdx.x & ~63)) * 16);
+        if (MODE == DX && second) {
+            if constexpr (IS_B) src.base[0] = (const char*)((const T*)o.p1 + row0);
+            else src.base[0] += a.half * (int64_t)sizeof(T);
         }
+#pragma unroll
+        for (int i = 0; i < BASES; ++i) src.base[i] += n * src.step;
+    }
+    // the next whole stage, direct global -> LDS at `lds` (+ the wave's share of it)
+    static __device__ __forceinline__ void load_direct(Source& src, int lds) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) load_to_lds(src.base[BASES == 1 ? 0 : i], src.off[i], lds + i * THREADS * 16);
+#pragma unroll
+        for (int i = 0; i < BASES; ++i) src.base[i] += src.step;
     }
     // ragged stage, through registers: zeros from k = K on and beyond the edges of across tiles
     static __device__ __forceinline__ void load_masked(const ProductArgs& a, int64_t row0, int64_t rows, int64_t k0, bool second, char* lds) {
@@ -215,32 +234,45 @@ struct Tile {
             *(Vec<T>*)(lds + (size_t)(i * THREADS + threadIdx.x) * 16) = load_part(p, left);
         }
     }
-    // the lane's operand of the 32 rows from `base` on for k step ks (16 elements of k, float32: 8)
-    static __device__ __forceinline__ typename Frag<T>::type frag(const char* lds, int base, int ks, int lane) {
+    // The lane's operands: byte offsets in a stage, found once, of `N` groups of 32 rows from `base` on
+    template <int N> struct Lane { int off[ACROSS ? N : 2]; };
+    template <int N> static __device__ __forceinline__ void place_lane(Lane<N>& l, int base, int lane, int tile) {
         if constexpr (!ACROSS) {
-            const int r = base + (lane & 31);
-            return *(const typename Frag<T>::type*)(lds + r * ROW_BYTES + tile_k_along(r, 2 * ks + (lane >> 5)) * 16);
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
+                l.off[ks] = tile + (base + (lane & 31)) * ROW_BYTES + tile_k_along(lane & 31, 2 * ks + (lane >> 5)) * 16;
+        } else {
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                if constexpr (sizeof(T) == 2) {
+                    const int g = lane >> 4, i = lane & 15, kr = 8 * (g >> 1) + (i >> 2);
+                    const int c = (base + 32 * n) / 8 + 2 * (g & 1) + ((i >> 1) & 1);
+                    l.off[n] = tile + kr * (ROWS * 2) + tile_k_across<T>(kr, c) * 16 + (i & 1) * 8;
+                } else {
+                    const int m = base + 32 * n + (lane & 31), kr = 4 * (lane >> 5);
+                    l.off[n] = tile + kr * (ROWS * 4) + tile_k_across<T>(kr, m >> 2) * 16 + (m & 3) * 4;
+                }
+            }
+        }
+    }
+    // operand of group n for k step ks (16 elements of k, float32: 8) of the stage at `lds`
+    template <int N> static __device__ __forceinline__ typename Frag<T>::type frag(const char* lds, const Lane<N>& l, int n, int ks) {
+        if constexpr (!ACROSS) {
+            return *(const typename Frag<T>::type*)(lds + l.off[ks] + n * 32 * ROW_BYTES);
         } else if constexpr (sizeof(T) == 2) {
-            const int g = lane >> 4, i = lane & 15;
-            const int c = base / 8 + 2 * (g & 1) + ((i >> 1) & 1);
             short8v out;
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const int kr = 16 * ks + 8 * (g >> 1) + 4 * half + (i >> 2);
-                const char* p = lds + kr * (ROWS * 2) + tile_k_across<T>(kr, c) * 16 + (i & 1) * 8;
+                const char* p = lds + l.off[n] + (16 * ks + 4 * half) * (ROWS * 2);
                 const short4v t = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)p);
 #pragma unroll
                 for (int s = 0; s < 4; ++s) out[4 * half + s] = t[s];
             }
             return out;
         } else {
-            const int m = base + (lane & 31);
             floatx4 out;
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const int kr = 8 * ks + 4 * (lane >> 5) + s;
-                out[s] = *(const float*)(lds + kr * (ROWS * 4) + tile_k_across<T>(kr, m >> 2) * 16 + (m & 3) * 4);
-            }
+            for (int s = 0; s < 4; ++s) out[s] = *(const float*)(lds + l.off[n] + (8 * ks + s) * (ROWS * 4));
             return out;
         }
     }
@@ -294,24 +326,40 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
     const int whole = (int)(args.K / BK), ragged = args.K % BK ? (MODE == DX ? 2 : 1) : 0, all = ragged + whole * (MODE == DX ? 2 : 1);
     const int first = blockIdx.y * args.stages, last = first + args.stages < all ? first + args.stages : all;
     floatx16 acc[MI][NI] = {};
-    typename TA::Pointers pa;
-    typename TB::Pointers pb;
-    TA::pointers(args, m0, args.M, pa);
-    TB::pointers(args, n0, args.N, pb);
-
-    auto load_whole = [&](int s, char* buf) {
-        const int q = s - ragged;
-        const bool second = MODE == DX && q >= whole;
-        const int64_t k0 = (int64_t)(second ? q - whole : q) * BK;
-        TA::load_direct(args, pa, k0, second, buf);
-        TB::load_direct(args, pb, k0, second, buf + A_BYTES);
+    typename TA::Source sa;
+    typename TB::Source sb;
+    TA::source(args, m0, args.M, sa);
+    TB::source(args, n0, args.N, sb);
+    const int wave_at = uniform((int)(uint32_t)(uintptr_t)(lds_char*)lds + wave * 1024);
+    // the next whole stage in line into place `at` of the ring; DX: number `whole` begins with the second pass
+    int next = first > ragged ? first - ragged : 0;
+    if (MODE == DX && next >= whole) {
+        TA::seek(args, m0, next - whole, true, sa);
+        TB::seek(args, n0, next - whole, true, sb);
+    } else {
+        TA::seek(args, m0, next, false, sa);
+        TB::seek(args, n0, next, false, sb);
+    }
+    auto load_whole = [&](int at) {
+        if (MODE == DX && next == whole && first - ragged < whole) {
+            sa.base[0] -= whole * sa.step;
+            TA::seek(args, m0, 0, true, sa);
+            TB::seek(args, n0, 0, true, sb);
+        }
+        TA::load_direct(sa, wave_at + at);
+        TB::load_direct(sb, wave_at + at + A_BYTES);
+        ++next;
     };
     typename Frag<T>::type fa[2][MI], fb[2][NI];
+    typename TA::template Lane<MI> la;
+    typename TB::template Lane<NI> lb;
+    TA::place_lane(la, wm * (BM / WM), lane, 0);
+    TB::place_lane(lb, wn * (BN / WN), lane, A_BYTES);
     auto read = [&](const char* buf, int ks) {
 #pragma unroll
-        for (int i = 0; i < MI; ++i) fa[ks][i] = TA::frag(buf, wm * (BM / WM) + 32 * i, ks, lane);
+        for (int i = 0; i < MI; ++i) fa[ks][i] = TA::frag(buf, la, i, ks);
 #pragma unroll
-        for (int j = 0; j < NI; ++j) fb[ks][j] = TB::frag(buf + A_BYTES, wn * (BN / WN) + 32 * j, ks, lane);
+        for (int j = 0; j < NI; ++j) fb[ks][j] = TB::frag(buf, lb, j, ks);
     };
     auto multiply = [&](int ks, int from, int to) {
 #pragma unroll
@@ -333,7 +381,7 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
     for (int t = 0; t < AHEAD && first + t < last; ++t) {
         const int s = first + t;
         char* buf = lds + t * BUF;
-        if (s >= ragged) load_whole(s, buf);
+        if (s >= ragged) load_whole(t * BUF);
         else {                                    // its loads are waited for at once, and with them all earlier ones
             TA::load_masked(args, m0, args.M, (int64_t)whole * BK, s == 1, buf);
             TB::load_masked(args, n0, args.N, (int64_t)whole * BK, s == 1, buf + A_BYTES);
@@ -350,7 +398,7 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
     for (int s = first; s < last; ++s) {
         const bool more = s + AHEAD < last;
         multiply(0, 0, 1);
-        if (more) load_whole(s + AHEAD, lds + fill);
+        if (more) load_whole(fill);
         read(lds + cur, 1);
         multiply(0, 1, MI);
         interleave(std::integral_constant<int, MI - 1>{});
@@ -589,10 +637,14 @@ int64_t round_256(int64_t n) { return (n + 255) / 256 * 256; }
 // Rows of `n` elements as the product kernel takes them: 16-byte aligned, whole chunks readable (what is behind a row's
 // end inside its last chunk meets only zeros or results that are not stored).
 struct Matrix { const void* p; int64_t ld, rows; };
-template <typename T> bool aligned(const Matrix& m, int64_t n) { return ((uintptr_t)m.p & 15) == 0 && m.ld % Chunk<T>::n == 0 && n % Chunk<T>::n == 0; }
+// (strides up to 2^21 elements: offsets inside a tile are 32-bit bytes)
+constexpr int64_t MAX_LD = 1 << 21;
+template <typename T> bool aligned(const Matrix& m, int64_t n) {
+    return ((uintptr_t)m.p & 15) == 0 && m.ld % Chunk<T>::n == 0 && n % Chunk<T>::n == 0 && m.ld <= MAX_LD;
+}
 template <typename T> int64_t packed_ld(int64_t n) { return (n + Chunk<T>::n - 1) / Chunk<T>::n * Chunk<T>::n; }
-template <typename T> size_t packed_bytes(const Matrix& m, int64_t n) {
-    return aligned<T>(m, n) ? 0 : (size_t)round_256(m.rows * packed_ld<T>(n) * (int64_t)sizeof(T));
+template <typename T> size_t packed_bytes(const Matrix& m, int64_t n, bool always = false) {
+    return aligned<T>(m, n) && !always ? 0 : (size_t)round_256(m.rows * packed_ld<T>(n) * (int64_t)sizeof(T));
 }
 template <typename T>
 __global__ __launch_bounds__(256) void pack_rows_kernel(const T* __restrict__ src, int64_t ld, T* __restrict__ dst, int64_t rows, int64_t n, int64_t per) {
@@ -602,8 +654,8 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(const T* __restrict__ sr
             *(Vec<T>*)(dst + (r * per + q) * CE) = load_part(src + r * ld + q * CE, n - q * CE);
 }
 // m itself, or its copy in the workspace (which moves on)
-template <typename T> Matrix pack(const Matrix& m, int64_t n, char*& ws, hipStream_t stream) {
-    const size_t bytes = packed_bytes<T>(m, n);
+template <typename T> Matrix pack(const Matrix& m, int64_t n, char*& ws, hipStream_t stream, bool always = false) {
+    const size_t bytes = packed_bytes<T>(m, n, always);
     if (bytes == 0) return m;
     const Matrix to = {ws, packed_ld<T>(n), m.rows};
     ws += bytes;
@@ -617,7 +669,8 @@ struct Gated { int64_t rows; int32_t d, h; Matrix x, wg, wu; };
 constexpr int FEW_ROWS = 64;              // up to here the forward product reads its operands as they are
 
 template <typename T> size_t workspace(const Gated& g, bool backward) {
-    const size_t packed = backward || g.rows > FEW_ROWS ? packed_bytes<T>(g.x, g.d) + packed_bytes<T>(g.wg, g.d) + packed_bytes<T>(g.wu, g.d) : 0;
+    const bool both = backward && (g.wg.ld != g.wu.ld || !aligned<T>(g.wg, g.d) || !aligned<T>(g.wu, g.d));
+    const size_t packed = backward || g.rows > FEW_ROWS ? packed_bytes<T>(g.x, g.d) + packed_bytes<T>(g.wg, g.d, both) + packed_bytes<T>(g.wu, g.d, both) : 0;
     if (!backward) return packed;
     const int64_t h2 = 2 * packed_ld<T>(g.h);
     const Plan px = plan_of<T>(DX, g.rows, g.d, g.h), pw = plan_of<T>(DW, h2, g.d, g.rows);
@@ -649,7 +702,11 @@ template <typename T> int backward(Gated g, const void* f, const void* p, const 
     hipLaunchKernelGGL(gated_da_db_kernel<T>, dim3((unsigned)((per + 255) / 256), (unsigned)(g.rows < 65535 ? g.rows : 65535)), dim3(256), 0, stream,
                        (const T*)f, (const T*)p, (const T*)gy, ldgy, dab, half, g.rows, (int64_t)g.h);
     hipError_t err = hipGetLastError();
-    if (err == hipSuccess && dx) { g.wg = pack<T>(g.wg, g.d, ws, stream); g.wu = pack<T>(g.wu, g.d, ws, stream); }
+    if (err == hipSuccess && dx) {                // DX moves through both weights with one stride
+        const bool both = g.wg.ld != g.wu.ld || !aligned<T>(g.wg, g.d) || !aligned<T>(g.wu, g.d);
+        g.wg = pack<T>(g.wg, g.d, ws, stream, both);
+        g.wu = pack<T>(g.wu, g.d, ws, stream, both);
+    }
     if (err == hipSuccess && dwg) g.x = pack<T>(g.x, g.d, ws, stream);
     float* partial = (float*)ws;
     if (err == hipSuccess && dx) {
@@ -675,7 +732,7 @@ int check_sizes(int32_t dtype, int32_t act, int64_t rows, int32_t d, int32_t h) 
     if (rows < 1 || d < 1 || h < 1) return MARL_EINVAL;
     if (dtype < MARL_F32 || dtype > MARL_F16 || act < MARL_ACT_SILU || act > MARL_ACT_SIGMOID) return MARL_EINVAL;
     // tile and block counts stay below 2^31
-    if (rows > (1ll << 31) - 256 || d > (1 << 24) || h > (1 << 24) || ((rows + 127) / 128) * (((int64_t)h + 31) / 32) > (1ll << 30) ||
+    if (rows > (1ll << 31) - 256 || d > (1 << 20) || h > (1 << 20) || ((rows + 127) / 128) * (((int64_t)h + 31) / 32) > (1ll << 30) ||
         ((rows + 127) / 128) * (((int64_t)d + 31) / 32) > (1ll << 30)) return MARL_EUNSUPPORTED;
     return MARL_OK;
 }
