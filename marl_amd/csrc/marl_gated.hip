@@ -340,16 +340,16 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
         TA::seek(args, m0, next, false, sa);
         TB::seek(args, n0, next, false, sb);
     }
-    auto load_whole = [&](int at) {
+    auto load_a = [&](int at) {
         if (MODE == DX && next == whole && first - ragged < whole) {
             sa.base[0] -= whole * sa.step;
             TA::seek(args, m0, 0, true, sa);
             TB::seek(args, n0, 0, true, sb);
         }
         TA::load_direct(sa, wave_at + at);
-        TB::load_direct(sb, wave_at + at + A_BYTES);
         ++next;
     };
+    auto load_b = [&](int at) { TB::load_direct(sb, wave_at + at + A_BYTES); };
     typename Frag<T>::type fa[2][MI], fb[2][NI];
     typename TA::template Lane<MI> la;
     typename TB::template Lane<NI> lb;
@@ -381,8 +381,10 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
     for (int t = 0; t < AHEAD && first + t < last; ++t) {
         const int s = first + t;
         char* buf = lds + t * BUF;
-        if (s >= ragged) load_whole(t * BUF);
-        else {                                    // its loads are waited for at once, and with them all earlier ones
+        if (s >= ragged) {
+            load_a(t * BUF);
+            load_b(t * BUF);
+        } else {                                    // its loads are waited for at once, and with them all earlier ones
             TA::load_masked(args, m0, args.M, (int64_t)whole * BK, s == 1, buf);
             TB::load_masked(args, n0, args.N, (int64_t)whole * BK, s == 1, buf + A_BYTES);
         }
@@ -390,26 +392,31 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
     wait_loads<LOADS>(last - first - 1);
     lds_barrier();
     read(lds, 0);
-    // One stage a turn: the products of its first half, among them the loads of the stage three ahead and the reads of its
-    // second half; the barrier; the products of the second half, which cover the first reads of the next stage.  A stage is
-    // loaded into the place of the one two before: what any wave read there it had used before the last barrier.  (The last
-    // turns load nothing, and the very last reads a half stage that it does not use.)
+    // One stage a turn: the products of its first half, among them A's loads of the stage three ahead and the reads of its
+    // second half; the barrier; the products of the second half, which cover the first reads of the next stage and B's
+    // loads (all loads at once behind the barrier: the waves hold each other up, 3 % slower).  A stage is loaded into the
+    // place of the one two before: what any wave read there it had used before the last barrier.  (The last turns load
+    // nothing, and the very last reads a half stage that it does not use.)
     int cur = 0, fill = AHEAD * BUF;
     for (int s = first; s < last; ++s) {
         const bool more = s + AHEAD < last;
         multiply(0, 0, 1);
-        if (more) load_whole(fill);
+        if (more) load_a(fill);
         read(lds + cur, 1);
         multiply(0, 1, MI);
         interleave(std::integral_constant<int, MI - 1>{});
-        fill = fill == (STAGES - 1) * BUF ? 0 : fill + BUF;
         cur = cur == (STAGES - 1) * BUF ? 0 : cur + BUF;
-        wait_loads<LOADS>(more ? AHEAD - 1 : 0);
+        // stage s + 1 is there when no more than the loads of s + 2 and half of those of s + 3 are under way
+        if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((AHEAD - 2) * LOADS + TA::PER) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
+        multiply(1, 0, 1);
+        if (more) load_b(fill);
+        fill = fill == (STAGES - 1) * BUF ? 0 : fill + BUF;
         read(lds + cur, 0);
-        multiply(1, 0, MI);
-        interleave(std::integral_constant<int, MI>{});
+        multiply(1, 1, MI);
+        interleave(std::integral_constant<int, MI - 1>{});
     }
     // Results through LDS, 32 rows of the wave at a time in a corner of its own: register v of a lane is row
     // 8 (v / 4) + 4 (lane / 32) + v % 4, column lane % 32; what leaves are 16-byte chunks of whole rows.
