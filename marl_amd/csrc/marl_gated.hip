@@ -223,15 +223,24 @@ struct Tile {
 #pragma unroll
         for (int i = 0; i < BASES; ++i) src.base[i] += src.step;
     }
-    // ragged stage, through registers: zeros from k = K on and beyond the edges of across tiles
+    // ragged stage, through registers: zeros from k = K on.  (Chunks are whole: rows along k are padded with zeros to whole
+    // chunks, what is behind the edge of an across row inside its last chunk is not stored.)
     static __device__ __forceinline__ void load_masked(const ProductArgs& a, int64_t row0, int64_t rows, int64_t k0, bool second, char* lds) {
+        Vec<T> v[PER];
+        bool in[PER];
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             int r, e;
             place(i * THREADS + (int)threadIdx.x, r, e);
-            const int64_t left = !ACROSS ? a.K - (k0 + e) : k0 + r < a.K ? rows - (row0 + e) : 0;
-            const T* p = row_ptr(a, row0, rows, left > 0 ? k0 : 0, left > 0 ? r : 0, second) + (ACROSS ? row0 + e : k0 + e);
-            *(Vec<T>*)(lds + (size_t)(i * THREADS + threadIdx.x) * 16) = load_part(p, left);
+            in[i] = ACROSS ? k0 + r < a.K && row0 + e < rows : k0 + e < a.K;
+            const int64_t kk = in[i] ? k0 : 0, col = !ACROSS ? (in[i] ? k0 + e : 0) : in[i] ? row0 + e : 0;
+            v[i] = load_chunk(row_ptr(a, row0, rows, kk, ACROSS && !in[i] ? 0 : r, second) + col);
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+#pragma unroll
+            for (int e = 0; e < CE; ++e) v[i].e[e] = in[i] ? v[i].e[e] : (T)0.0f;
+            *(Vec<T>*)(lds + (size_t)(i * THREADS + threadIdx.x) * 16) = v[i];
         }
     }
     // The lane's operands: byte offsets in a stage, found once, of `N` groups of 32 rows from `base` on
@@ -517,11 +526,10 @@ __global__ __launch_bounds__(512) void gated_few_rows_kernel(const ProductArgs a
         } else {
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                const int64_t left = d - (k + c * CE);
-                g[c] = load_part(wg + k + c * CE, left);
-                u[c] = load_part(wu + k + c * CE, left);
+                g[c] = load_clipped(wg, k + c * CE, d);
+                u[c] = load_clipped(wu, k + c * CE, d);
 #pragma unroll
-                for (int i = 0; i < MT; ++i) xv[i][c] = load_part(x[i] + k + c * CE, left);
+                for (int i = 0; i < MT; ++i) xv[i][c] = load_clipped(x[i], k + c * CE, d);
             }
         }
 #pragma unroll
@@ -561,7 +569,7 @@ __global__ __launch_bounds__(512) void gated_few_rows_kernel(const ProductArgs a
     });
 }
 
-// da = gy p and, `half` columns behind it, db = gy f of every row: bandwidth (three reads, two writes of T h)
+// da = gy p and, `half` columns behind it, db = gy f of every row, both padded with zeros: bandwidth (three reads, two writes of T h)
 template <typename T>
 __global__ __launch_bounds__(256) void gated_da_db_kernel(const T* __restrict__ f, const T* __restrict__ p, const T* __restrict__ gy, int64_t ldgy,
                                                            T* __restrict__ dab, int64_t half, int64_t rows, int64_t h) {
@@ -569,8 +577,8 @@ __global__ __launch_bounds__(256) void gated_da_db_kernel(const T* __restrict__ 
     const int64_t per = (h + CE - 1) / CE;
     for (int64_t t = blockIdx.y; t < rows; t += gridDim.y)
         for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < per; q += (int64_t)gridDim.x * 256) {
-            const int64_t c = q * CE, left = h - c;
-            const Vec<T> vf = load_part(f + t * h + c, left), vp = load_part(p + t * h + c, left), vg = load_part(gy + t * ldgy + c, left);
+            const int64_t c = q * CE;
+            const Vec<T> vf = load_clipped(f + t * h, c, h), vp = load_clipped(p + t * h, c, h), vg = load_clipped(gy + t * ldgy, c, h);
             Vec<T> da, db;
 #pragma unroll
             for (int i = 0; i < CE; ++i) {
@@ -578,8 +586,8 @@ __global__ __launch_bounds__(256) void gated_da_db_kernel(const T* __restrict__ 
                 da.e[i] = from_f32<T>(g * to_f32(vp.e[i]));
                 db.e[i] = from_f32<T>(g * to_f32(vf.e[i]));
             }
-            store_part(dab + t * 2 * half + c, da, left);
-            store_part(dab + t * 2 * half + half + c, db, left);
+            *(Vec<T>*)(dab + t * 2 * half + c) = da;                // zeros behind h
+            *(Vec<T>*)(dab + t * 2 * half + half + c) = db;
         }
 }
 
@@ -641,8 +649,7 @@ template <typename T, int MT> hipError_t launch_few_rows(const ProductArgs& a, h
 
 int64_t round_256(int64_t n) { return (n + 255) / 256 * 256; }
 
-// Rows of `n` elements as the product kernel takes them: 16-byte aligned, whole chunks readable (what is behind a row's
-// end inside its last chunk meets only zeros or results that are not stored).
+// Rows of `n` elements as the product kernel takes them: 16-byte aligned, the last chunk whole, with zeros behind the row's end.
 struct Matrix { const void* p; int64_t ld, rows; };
 // (strides up to 2^21 elements: offsets inside a tile are 32-bit bytes)
 constexpr int64_t MAX_LD = 1 << 21;
@@ -658,7 +665,7 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(const T* __restrict__ sr
     constexpr int CE = Chunk<T>::n;
     for (int64_t r = blockIdx.y; r < rows; r += gridDim.y)
         for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < per; q += (int64_t)gridDim.x * 256)
-            *(Vec<T>*)(dst + (r * per + q) * CE) = load_part(src + r * ld + q * CE, n - q * CE);
+            *(Vec<T>*)(dst + (r * per + q) * CE) = load_clipped(src + r * ld, q * CE, n);
 }
 // m itself, or its copy in the workspace (which moves on)
 template <typename T> Matrix pack(const Matrix& m, int64_t n, char*& ws, hipStream_t stream, bool always = false) {

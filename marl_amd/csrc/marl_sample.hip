@@ -201,14 +201,106 @@ __device__ __forceinline__ double wave_before(double v, int lane) {
     return s - v;
 }
 
+// bits of an ordered value below which all keys of one sign are equal: ones for negative values, zeros for others
+template <typename T> struct LowBits { static constexpr int n = sizeof(T) == 4 ? 0 : std::is_same<T, bf16>::value ? 16 : 13; };
+
+// the first `take` of the elements equal to `key`, in index order, are kept, those above all, the others lose their weight
+template <int N> __device__ __forceinline__ void keep_above(const float (&l)[N], double (&w)[N], uint32_t key, int take, int lane) {
+    int mine = 0;
+#pragma unroll
+    for (int e = 0; e < N; ++e) mine += key_of(l[e]) == key;
+    int before = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) { const int t = __shfl_up(before, o); if (lane >= o) before += t; }
+    before -= mine;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        const uint32_t k = key_of(l[e]);
+        if (k < key || (k == key && before >= take)) w[e] = 0.0;
+        before += k == key;
+    }
+}
+
+// top-p, min-p and the draw among N weighted elements a lane, in index order over lanes and elements
+template <typename T, int N, class Index>
+__device__ __forceinline__ void finish_row(const SampleArgs& a, int64_t r, const Rule& rule, float top, const float (&l)[N], double (&w)[N], int lane, Index&& index_of) {
+    constexpr int LOW = LowBits<T>::n;
+    constexpr uint32_t ONES = (1u << LOW) - 1;
+    if (rule.p < 1.0) {
+        double sum = 0.0;
+        uint32_t least = 0xFFFFFFFFu;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            sum += w[e];
+            const uint32_t k = key_of(l[e]);
+            if (w[e] > 0.0 && k < least) least = k;
+        }
+        double goal = rule.p * wave_sum(sum);
+        goal = goal > 1.0 ? goal : 1.0;
+#pragma unroll
+        for (int o = 32; o > 0; o /= 2) { const uint32_t t = (uint32_t)__shfl_xor((int)least, o); least = t < least ? t : least; }
+        // key: the largest with a mass of at least `goal` at or above it.  It lies between the smallest weighted value and
+        // the maximum, whose common bits it shares.
+        const uint32_t most = key_of(top), differ = most ^ least;
+        const int high = differ ? 31 - __clz((int)differ) : -1;
+        uint32_t key = high >= 31 ? 0 : most & ~((2u << (high < 0 ? 0 : high)) - 1u);
+        if (high < 0) key = most;
+#pragma unroll 1
+        for (int bit = high; bit >= LOW; --bit) {
+            const uint32_t c = key | (1u << bit);
+            double m = 0.0;
+#pragma unroll
+            for (int e = 0; e < N; ++e) m += (key_of(l[e]) | ONES) >= (c | ONES) ? w[e] : 0.0;
+            if (wave_sum(m) >= goal) key = c;
+        }
+        double above = 0.0, one = 0.0;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const uint32_t k = key_of(l[e]) | ONES;
+            above += k > (key | ONES) ? w[e] : 0.0;
+            if (k == (key | ONES)) one = fmax(one, w[e]);
+        }
+        above = wave_sum(above);
+#pragma unroll
+        for (int o = 32; o > 0; o /= 2) one = fmax(one, __shfl_xor(one, o));
+        // the smallest number of them that reaches the goal (at least one)
+        double take = ceil((goal - above) / one);
+        if (take > 1.0 && above + (take - 1.0) * one >= goal) take -= 1.0;
+        if (above + take * one < goal) take += 1.0;
+        keep_above<N>(l, w, key & 0x80000000u ? key & ~ONES : key | ONES, take > 1.0 ? (int)fmin(take, 4096.0) : 1, lane);
+    }
+    double sum = 0.0;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        if (scaled(l[e], top, rule.inv_t) < rule.log_m) w[e] = 0.0;
+        sum += w[e];
+    }
+    double run = wave_before(sum, lane);
+    const double total = __shfl(run + sum, 63), target = target_of(a, r, total);
+    if (run <= target && run + sum > target) {
+        bool found = false;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            run += w[e];
+            if (!found && run > target) {
+                found = true;
+                a.index[r] = index_of(e);
+                a.log_prob[r] = log_prob_of(scaled(l[e], top, rule.inv_t), (u64)total);
+            }
+        }
+    }
+}
+
 template <typename T, int NE>
 __global__ __launch_bounds__(256) void sample_wave_kernel(const SampleArgs a) {
     constexpr int CE = Chunk<T>::n;
     __shared__ double pow64[64];
+    __shared__ float kept_l[4][64];
+    __shared__ int kept_i[4][64];
     if (threadIdx.x < 64) pow64[threadIdx.x] = kPow64[threadIdx.x];
     __syncthreads();
-    const int lane = threadIdx.x & 63;
-    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t r = (int64_t)blockIdx.x * 4 + wave;
     if (r >= a.rows) return;
     const T* row = (const T*)a.logits + r * a.ld;
     const Rule rule = rule_of(a, r);
@@ -217,7 +309,7 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(const SampleArgs a) {
     if constexpr (NE >= CE) {
 #pragma unroll
         for (int c = 0; c < NE; c += CE) {
-            const Vec<T> v = load_part(row + (left > c ? at + c : 0), left - c);
+            const Vec<T> v = load_clipped(row, (int64_t)at + c, (int64_t)a.V);
 #pragma unroll
             for (int e = 0; e < CE; ++e) l[c + e] = left > c + e ? clean(to_f32(v.e[e])) : -HUGE_VALF;
         }
@@ -244,28 +336,11 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(const SampleArgs a) {
     }
     double w[NE];
 #pragma unroll
-    for (int e = 0; e < NE; ++e) w[e] = weight_f64(scaled(l[e], top, rule.inv_t), pow64);
-    // the first `take` of the elements equal to `key`, in index order, are kept, those above all, the others lose their weight
-    auto keep = [&](uint32_t key, int take) {
-        int mine = 0;
-#pragma unroll
-        for (int e = 0; e < NE; ++e) mine += key_of(l[e]) == key;
-        int before = mine;
-#pragma unroll
-        for (int o = 1; o < 64; o *= 2) { const int t = __shfl_up(before, o); if (lane >= o) before += t; }
-        before -= mine;
-#pragma unroll
-        for (int e = 0; e < NE; ++e) {
-            const uint32_t k = key_of(l[e]);
-            if (k < key || (k == key && before >= take)) w[e] = 0.0;
-            before += k == key;
-        }
-    };
-    constexpr int LOW = sizeof(T) == 4 ? 0 : std::is_same<T, bf16>::value ? 16 : 13;      // bits below are equal in every key of a sign
-    // keys of negative values have ones there: a candidate is compared with them all set
-    constexpr uint32_t ONES = (1u << LOW) - 1;
+    for (int e = 0; e < NE; ++e) w[e] = 1.0;                // top-k needs no weights: a mark of what is left
     if (rule.k > 0) {
-        uint32_t key = 0;                       // the largest with at least k elements at or above it
+        constexpr int LOW = LowBits<T>::n;
+        constexpr uint32_t ONES = (1u << LOW) - 1;
+        uint32_t key = 0;                       // the largest with at least k elements at or above it, or one with exactly k
 #pragma unroll 1
         for (int bit = 31; bit >= LOW; --bit) {
             const uint32_t c = key | (1u << bit);
@@ -273,63 +348,35 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(const SampleArgs a) {
 #pragma unroll
             for (int e = 0; e < NE; ++e) n += __popcll(__ballot((key_of(l[e]) | ONES) >= (c | ONES)));
             if (n >= rule.k) key = c;
+            if (n == rule.k) break;
         }
         int above = 0;
 #pragma unroll
         for (int e = 0; e < NE; ++e) above += __popcll(__ballot((key_of(l[e]) | ONES) > (key | ONES)));
-        keep(key & 0x80000000u ? key : key | ONES, rule.k - above);
-    }
-    if (rule.p < 1.0) {
-        double sum = 0.0;
+        keep_above<NE>(l, w, key & 0x80000000u ? key & ~ONES : key | ONES, rule.k - above, lane);
+        if (rule.k <= 64) {                     // one element a lane from here on, still in index order
+            int mine = 0;
 #pragma unroll
-        for (int e = 0; e < NE; ++e) sum += w[e];
-        double goal = rule.p * wave_sum(sum);
-        goal = goal > 1.0 ? goal : 1.0;
-        uint32_t key = 0;                       // the largest with a mass of at least `goal` at or above it
-#pragma unroll 1
-        for (int bit = 31; bit >= LOW; --bit) {
-            const uint32_t c = key | (1u << bit);
-            double m = 0.0;
+            for (int e = 0; e < NE; ++e) mine += w[e] > 0.0;
+            int to = mine;
 #pragma unroll
-            for (int e = 0; e < NE; ++e) m += (key_of(l[e]) | ONES) >= (c | ONES) ? w[e] : 0.0;
-            if (wave_sum(m) >= goal) key = c;
-        }
-        double above = 0.0, each_ = 0.0;
+            for (int o = 1; o < 64; o *= 2) { const int t = __shfl_up(to, o); if (lane >= o) to += t; }
+            const int n = __shfl(to, 63);
+            to -= mine;
 #pragma unroll
-        for (int e = 0; e < NE; ++e) {
-            const uint32_t k = key_of(l[e]) | ONES;
-            above += k > (key | ONES) ? w[e] : 0.0;
-            if (k == (key | ONES)) each_ = fmax(each_, w[e]);
-        }
-        above = wave_sum(above);
-#pragma unroll
-        for (int o = 32; o > 0; o /= 2) each_ = fmax(each_, __shfl_xor(each_, o));
-        // the smallest number of them that reaches the goal (at least one)
-        double take = ceil((goal - above) / each_);
-        if (take > 1.0 && above + (take - 1.0) * each_ >= goal) take -= 1.0;
-        if (above + take * each_ < goal) take += 1.0;
-        keep(key & 0x80000000u ? key : key | ONES, take > 1.0 ? (int)fmin(take, 4096.0) : 1);
-    }
-    double sum = 0.0;
-#pragma unroll
-    for (int e = 0; e < NE; ++e) {
-        if (scaled(l[e], top, rule.inv_t) < rule.log_m) w[e] = 0.0;
-        sum += w[e];
-    }
-    double run = wave_before(sum, lane);
-    const double total = __shfl(run + sum, 63), target = target_of(a, r, total);
-    if (run <= target && run + sum > target) {
-        bool found = false;
-#pragma unroll
-        for (int e = 0; e < NE; ++e) {
-            run += w[e];
-            if (!found && run > target) {
-                found = true;
-                a.index[r] = at + e;
-                a.log_prob[r] = log_prob_of(scaled(l[e], top, rule.inv_t), (u64)total);
-            }
+            for (int e = 0; e < NE; ++e)
+                if (w[e] > 0.0) { kept_l[wave][to] = l[e]; kept_i[wave][to] = at + e; ++to; }
+            __builtin_amdgcn_wave_barrier();            // one wave: its LDS accesses are done in order
+            float l1[1] = {lane < n ? kept_l[wave][lane] : -HUGE_VALF};
+            const int i1 = lane < n ? kept_i[wave][lane] : 0;
+            double w1[1] = {weight_f64(scaled(l1[0], top, rule.inv_t), pow64)};
+            finish_row<T, 1>(a, r, rule, top, l1, w1, lane, [&](int) { return i1; });
+            return;
         }
     }
+#pragma unroll
+    for (int e = 0; e < NE; ++e) w[e] = w[e] > 0.0 ? weight_f64(scaled(l[e], top, rule.inv_t), pow64) : 0.0;
+    finish_row<T, NE>(a, r, rule, top, l, w, lane, [&](int e) { return at + e; });
 }
 
 // -- longer rows: a workgroup per row ----------------------------------------------------------------------------------

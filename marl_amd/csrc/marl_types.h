@@ -48,7 +48,23 @@ template <typename T> __device__ __forceinline__ void store_part(T* p, const Vec
     for (int i = 0; i < n; ++i) if (i < left) p[i] = v.e[i];
 }
 
-// the same for results that nothing reads soon: past the caches
+// The chunk of a row of n elements that begins at element c, zeros from n on.  Rows of a chunk or more: the last whole chunk
+// is loaded where c lies past it, and moved; no branch, whose loads would be waited for one by one.
+template <typename T> __device__ __forceinline__ Vec<T> load_clipped(const T* row, int64_t c, int64_t n) {
+    constexpr int CE = Chunk<T>::n;
+    if (n < CE) return load_part(row + (c < n ? c : 0), n - c);
+    const int64_t at = c < n - CE ? c : n - CE;
+    Vec<T> v = load_chunk(row + at);
+    const int by = c - at < CE ? (int)(c - at) : CE;
+#pragma unroll
+    for (int step = 1; step < CE; step *= 2)
+#pragma unroll
+        for (int e = 0; e < CE; ++e) v.e[e] = (by & step) && e + step < CE ? v.e[e + step] : v.e[e];
+#pragma unroll
+    for (int e = 0; e < CE; ++e) v.e[e] = e + by < CE ? v.e[e] : (T)0.0f;
+    return v;
+}
+// store_part for results that nothing reads soon: past the caches
 template <typename T> __device__ __forceinline__ void stream_part(T* p, const Vec<T>& v, int64_t left) {
     constexpr int n = Chunk<T>::n;
     if (left >= n) { __builtin_nontemporal_store(__builtin_bit_cast(uint4v, v), &((Unaligned*)p)->v); return; }
