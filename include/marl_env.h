@@ -482,8 +482,8 @@ enum { MARL_NORM_RMS = 0, MARL_NORM_LAYER = 1 };
 
 /* y[t][j] = act(a[t][j]) b[t][j],  a = x w_gate^T,  b = x w_up^T;  x [rows][d], weights [h][d], y [rows][h] contiguous.
  * f, p: both NULL, or [rows][h] contiguous buffers that receive act(a) and b act'(a) for the backward call.
- * workspace: 16-byte aligned, marl_gated_workspace_bytes of the same operands (backward 0; NULL where that is 0: rows that
- * are 16-byte aligned need none). */
+ * workspace: 16-byte aligned, marl_gated_workspace_bytes of the same operands (backward 0; NULL where that is 0: 16-byte
+ * aligned rows of more than 64, or of weights with many rows, need none). */
 int marl_gated_forward(int32_t dtype, int32_t act, int64_t rows, int32_t d, int32_t h, const void *x, int64_t ldx,
                        const void *w_gate, int64_t ld_gate, const void *w_up, int64_t ld_up, void *y, void *f, void *p,
                        void *workspace, void *stream);

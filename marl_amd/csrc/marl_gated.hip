@@ -495,7 +495,8 @@ __global__ __launch_bounds__(256) void sum_slices_kernel(const float* __restrict
 // Few rows (T <= 32 MT): the weights are read once and nothing else counts.  A block owns 32 columns j (rows of both
 // weights), its eight waves split d; a lane reads 64 consecutive bytes of one weight row and of one row of x, straight
 // into matrix operands (the order of k inside a run is the same for both, so it needs no shuffle).  The eight partial
-// sums meet in LDS.
+// sums meet in LDS.  Narrow weights leave most CUs without a block: d is then cut into slices over blocks too, whose sums
+// of a and b go to partial [slices][rows][2][h] and are finished by a second launch (5 x 3337 x 80 f16: 41 -> 22 us).
 template <typename T, int MT>
 __global__ __launch_bounds__(512) void gated_few_rows_kernel(const ProductArgs args) {
     constexpr int CE = Chunk<T>::n, RUN = 8 * CE, WAVES = 8;                // 4 chunks per half wave
@@ -513,7 +514,7 @@ __global__ __launch_bounds__(512) void gated_few_rows_kernel(const ProductArgs a
         x[i] = (const T*)args.A.p0 + t * args.A.ld0;
     }
     floatx16 acc[MT][2] = {};
-    for (int64_t k0 = (int64_t)wave * RUN; k0 < d; k0 += WAVES * RUN) {
+    for (int64_t k0 = ((int64_t)blockIdx.y * WAVES + wave) * RUN; k0 < d; k0 += (int64_t)gridDim.y * WAVES * RUN) {
         const int64_t k = k0 + hl * 4 * CE;
         Vec<T> g[4], u[4], xv[MT][4];
         if (k0 + RUN <= d) {
@@ -564,9 +565,32 @@ __global__ __launch_bounds__(512) void gated_few_rows_kernel(const ProductArgs a
                     a[e] += part[(((w * MT + t / 32) * 2 + 0) * 16 + v) * 64 + 32 * half + c + e];
                     b[e] += part[(((w * MT + t / 32) * 2 + 1) * 16 + v) * 64 + 32 * half + c + e];
                 }
-            gate_out<T, ACT>(args, t * args.N + j0 + c, a, b, args.N - (j0 + c));
+            if (args.partial == nullptr) {
+                gate_out<T, ACT>(args, t * args.N + j0 + c, a, b, args.N - (j0 + c));
+                continue;
+            }
+            float* out = args.partial + (((int64_t)blockIdx.y * args.M + t) * 2) * args.N + j0 + c;
+#pragma unroll
+            for (int e = 0; e < CE; ++e)
+                if (j0 + c + e < args.N) { out[e] = a[e]; out[args.N + e] = b[e]; }
         }
     });
+}
+// y (f, p) from the sums of a and b over the slices of d
+template <typename T>
+__global__ __launch_bounds__(256) void gated_finish_kernel(const ProductArgs args, int slices) {
+    constexpr int CE = Chunk<T>::n;
+    const int64_t per = (args.N + CE - 1) / CE, q = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (q >= args.M * per) return;
+    const int64_t t = q / per, j = q % per * CE;
+    float a[CE] = {}, b[CE] = {};
+    for (int z = 0; z < slices; ++z) {
+        const float* in = args.partial + (((int64_t)z * args.M + t) * 2) * args.N + j;
+#pragma unroll
+        for (int e = 0; e < CE; ++e)
+            if (j + e < args.N) { a[e] += in[e]; b[e] += in[args.N + e]; }
+    }
+    by_act(args.act, [&](auto kind) { gate_out<T, decltype(kind)::value>(args, t * args.N + j, a, b, args.N - j); });
 }
 
 // da = gy p and, `half` columns behind it, db = gy f of every row, both padded with zeros: bandwidth (three reads, two writes of T h)
@@ -638,12 +662,25 @@ hipError_t launch_product(ProductArgs& a, float* partial, hipStream_t stream) {
     return hipGetLastError();
 }
 
-template <typename T, int MT> hipError_t launch_few_rows(const ProductArgs& a, hipStream_t stream) {
+// slices of d over blocks: fewer than 64 blocks of columns, and a run for every wave of every slice
+template <typename T> int few_rows_slices(int64_t d, int64_t h) {
+    const int64_t blocks = (h + 31) / 32, most = d / (64 * Chunk<T>::n);
+    if (blocks >= 64 || most < 2) return 1;
+    return (int)(128 / blocks < most ? 128 / blocks : most);
+}
+
+template <typename T, int MT> hipError_t launch_few_rows(ProductArgs& a, void* ws, hipStream_t stream) {
     static bool attr_set[marl_net::kMaxDevices];
     const size_t bytes = (size_t)8 * MT * 2 * 16 * 64 * sizeof(float);
     hipError_t err = marl_net::allow_dynamic_lds((const void*)gated_few_rows_kernel<T, MT>, bytes, attr_set);
     if (err != hipSuccess) return err;
-    hipLaunchKernelGGL((gated_few_rows_kernel<T, MT>), dim3((unsigned)((a.N + 31) / 32)), dim3(512), bytes, stream, a);
+    const int slices = few_rows_slices<T>(a.K, a.N);
+    a.partial = slices > 1 ? (float*)ws : nullptr;
+    hipLaunchKernelGGL((gated_few_rows_kernel<T, MT>), dim3((unsigned)((a.N + 31) / 32), slices), dim3(512), bytes, stream, a);
+    if (slices > 1) {
+        const int64_t n = a.M * ((a.N + Chunk<T>::n - 1) / Chunk<T>::n);
+        hipLaunchKernelGGL(gated_finish_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, a, slices);
+    }
     return hipGetLastError();
 }
 
@@ -685,7 +722,10 @@ constexpr int FEW_ROWS = 64;              // up to here the forward product read
 template <typename T> size_t workspace(const Gated& g, bool backward) {
     const bool both = backward && (g.wg.ld != g.wu.ld || !aligned<T>(g.wg, g.d) || !aligned<T>(g.wu, g.d));
     const size_t packed = backward || g.rows > FEW_ROWS ? packed_bytes<T>(g.x, g.d) + packed_bytes<T>(g.wg, g.d, both) + packed_bytes<T>(g.wu, g.d, both) : 0;
-    if (!backward) return packed;
+    if (!backward) {
+        const int slices = g.rows <= FEW_ROWS ? few_rows_slices<T>(g.d, g.h) : 1;
+        return packed + (slices > 1 ? (size_t)slices * g.rows * 2 * g.h * sizeof(float) : 0);
+    }
     const int64_t h2 = 2 * packed_ld<T>(g.h);
     const Plan px = plan_of<T>(DX, g.rows, g.d, g.h), pw = plan_of<T>(DW, h2, g.d, g.rows);
     const int64_t sx = px.slices > 1 ? px.slices * g.rows * g.d : 0, sw = pw.slices > 1 ? pw.slices * h2 * g.d : 0;
@@ -700,7 +740,7 @@ template <typename T> int forward(int act, Gated g, void* y, void* f, void* p, v
     a.B = {g.wg.p, g.wu.p, g.wg.ld, g.wu.ld};
     a.M = g.rows; a.N = g.h; a.K = g.d; a.h = g.h;
     a.out0 = y; a.save_f = f; a.save_p = p; a.act = act;
-    const hipError_t err = g.rows <= 32 ? launch_few_rows<T, 1>(a, stream) : g.rows <= FEW_ROWS ? launch_few_rows<T, 2>(a, stream)
+    const hipError_t err = g.rows <= 32 ? launch_few_rows<T, 1>(a, workspace, stream) : g.rows <= FEW_ROWS ? launch_few_rows<T, 2>(a, workspace, stream)
                                                                                                 : launch_product<T, FWD>(a, nullptr, stream);
     if (err == hipSuccess) return MARL_OK;
     marl_note_hip_error((int)err);

@@ -900,23 +900,35 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(const SampleArgs a)
     }
 }
 
-template <typename T> int run(const SampleArgs& a, hipStream_t stream) {
+template <typename T> void launch(const SampleArgs& a, hipStream_t stream) {
 #define MARL_SHORT(L) hipLaunchKernelGGL((sample_short_kernel<T, L>), dim3((unsigned)((a.rows + 256 / L - 1) / (256 / L))), dim3(256), 0, stream, a)
+#define MARL_WAVE(NE) hipLaunchKernelGGL((sample_wave_kernel<T, NE>), dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, stream, a)
     if (a.V <= 4) MARL_SHORT(4);
     else if (a.V <= 8) MARL_SHORT(8);
     else if (a.V <= 16) MARL_SHORT(16);
     else if (a.V <= 32) MARL_SHORT(32);
     else if (a.V <= 64) MARL_SHORT(64);
-#undef MARL_SHORT
-#define MARL_WAVE(NE) hipLaunchKernelGGL((sample_wave_kernel<T, NE>), dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, stream, a)
     else if (a.V <= 128) MARL_WAVE(2);
     else if (a.V <= 256) MARL_WAVE(4);
     else if (a.V <= 512) MARL_WAVE(8);
     else if (a.V <= 1024) MARL_WAVE(16);
     else if (a.V <= 2048) MARL_WAVE(32);
-#undef MARL_WAVE
     else if (a.V <= 8192) hipLaunchKernelGGL((sample_row_kernel<T, 256>), dim3((unsigned)a.rows), dim3(256), 0, stream, a);
     else hipLaunchKernelGGL((sample_row_kernel<T, 1024>), dim3((unsigned)a.rows), dim3(1024), 0, stream, a);
+#undef MARL_SHORT
+#undef MARL_WAVE
+}
+
+template <typename T> int run(const SampleArgs& all, hipStream_t stream) {
+    constexpr int64_t MOST = 1 << 21;              // rows of a launch: its threads stay below 2^32
+    for (int64_t first = 0; first < all.rows; first += MOST) {
+        SampleArgs a = all;
+        a.logits = (const T*)all.logits + first * all.ld;
+        a.rows = all.rows - first < MOST ? all.rows - first : MOST;
+        a.u += first; a.index += first; a.log_prob += first;
+        if (a.settings) a.settings += 4 * first;
+        launch<T>(a, stream);
+    }
     const hipError_t err = hipGetLastError();
     if (err == hipSuccess) return MARL_OK;
     marl_note_hip_error((int)err);

@@ -119,6 +119,26 @@ def test_gated_linear_large_tiles(dt, T, d, h):
     gated_check(T, d, h, dt, "silu", seed=5)
 
 
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+@pytest.mark.parametrize("T,d,h", [(1, 1024, 33), (5, 3337, 80), (40, 2050, 7), (64, 1536, 2016), (2, 4096, 1)])
+def test_gated_linear_few_rows_over_narrow_weights(T, d, h, dt):
+    """The slices of d over blocks, and both sides of where they begin."""
+    gated_check(T, d, h, dt, "silu", seed=d)
+
+
+def test_gated_linear_weights_of_different_strides():
+    """Rows of w_gate and w_up spaced differently: the gradient of x moves through both."""
+    rn = gen(12)
+    x, wg, wu, gy = rn(150, 64), rn(72, 64) / 8, rn(72, 64) / 8, rn(150, 72)
+    want, tol = gated_oracle(x, wg, wu, gy, "silu")
+    wide = torch.full((72, 96), float("nan"), device="cuda")
+    wide[:, :64] = wu
+    leaves = [x.cuda().requires_grad_(True), wg.cuda().requires_grad_(True), wide[:, :64].detach().requires_grad_(True)]
+    y = ops.gated_linear(*leaves)
+    for g, w, t in zip((y,) + torch.autograd.grad(y, leaves, gy.cuda()), want, tol):
+        close("strides", g, w, t)
+
+
 @pytest.mark.parametrize("dt", [F32, BF16])
 @pytest.mark.parametrize("T", [7, 140])
 def test_gated_linear_strided_and_shifted_operands(dt, T):
@@ -523,6 +543,32 @@ def test_sample_logits_frequencies_follow_the_weights():
     share = torch.bincount(index.cpu(), minlength=4).double() / R
     assert float((share - p).abs().max()) < 5 * (0.25 / R) ** 0.5                 # five standard deviations
     assert float((lp.cpu() - p.log()[index.cpu()]).abs().max()) < 1e-6            # float32 logs of the weights
+
+
+def test_sample_logits_more_rows_than_one_launch_takes():
+    R = (1 << 21) + 3
+    u = torch.rand(R, device="cuda")
+    logits = torch.zeros(R, 2, device="cuda")
+    logits[:, 1] = torch.where(torch.arange(R, device="cuda") % 3 == 0, float("-inf"), 0.0)
+    index, lp = ops.sample_logits(logits, u)
+    open_ = logits[:, 1] == 0.0
+    assert torch.equal(index, (open_ & (u >= 0.5)).long())          # u 2 is exact: 1 exceeds it below a half
+    half = torch.tensor(0.5).log().item()
+    assert float((lp - torch.where(open_, half, 0.0)).abs().max()) < 1e-7
+
+
+def test_second_gradients():
+    """keyed_dropout is linear and differentiable again; the others say that they are not."""
+    x = torch.randn(5, 24, device="cuda", requires_grad=True)
+    c = torch.randn(5, 24, device="cuda", requires_grad=True)
+    g, = torch.autograd.grad((ops.keyed_dropout(x, 0.5, 3) * c).sum(), x, create_graph=True)
+    gg, = torch.autograd.grad((g * 2.0).sum(), c)
+    assert torch.equal(gg, ops.keyed_dropout(torch.full_like(x, 2.0), 0.5, 3))
+    w = torch.randn(8, 24, device="cuda", requires_grad=True)
+    for f in (lambda: ops.gated_linear(x, w, w), lambda: ops.residual_norm(x, x, c[0], c[1])[1]):
+        g, = torch.autograd.grad(f().pow(2).sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            g.sum().backward()
 
 
 def test_sample_logits_strides_and_shapes():
