@@ -13,7 +13,7 @@
 // borders of top-k and top-p are found by bisection over the bits of the ordered values, a count (ballots) or a sum each.
 // Longer rows: a workgroup per row, which
 // reads its row a few times (the first time from HBM, then from L2).  With a small top-k, twice: the maximum, and every
-// thread's own; k threads have a maximum above the k-th largest of those, so no element below it can be among the first k;
+// thread's own two largest; k elements are above the k-th largest of those, so none below it can be among the first k;
 // the few elements above are sorted in LDS and the rest happens there.  Otherwise: maximum; counts and masses over bins
 // of a fraction of a nat below the maximum; the elements of the bin in which a border falls, sorted in LDS; the masses of
 // the kept.
@@ -380,9 +380,13 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(const SampleArgs a) {
 }
 
 // -- longer rows: a workgroup per row ----------------------------------------------------------------------------------
-// The workgroups: 1024 threads for the longest rows (one or two to a CU); 256 with a quarter of the LDS for shorter ones.
+// The workgroups: 1024 threads (one to a CU) for long rows if there are few, 256 for shorter rows and for many: what a row
+// takes is mostly waiting, for its loads and at barriers (981 x 34 183 f16, top-k 64 and top-p: 74 us with 1024 threads).
+// With 256, registers are held to six workgroups a CU; left free, the kernel takes more than 128 and two fit (same call,
+// two : four : six a CU: 52 : 37 : 37 us; 4096 x 3000: 116 : 65 : 52; top-p alone, where six spill, 219 : 159 : 162).
 template <int THREADS> struct Dim {
-    static constexpr int BINS = THREADS == 1024 ? 2048 : 512, CAP = BINS;        // bins; elements sorted at once
+    static constexpr int BINS = THREADS == 1024 ? 2048 : 512;                    // bins
+    static constexpr int CAP = THREADS == 1024 ? 2048 : 1024;                    // elements sorted at once
     static constexpr double PER_NAT = BINS / 32.0;                               // the bins cover 32 nats
 };
 
@@ -662,17 +666,18 @@ __device__ __noinline__ Cut cut_of(Shared<THREADS>& s, const T* row, int32_t V, 
     return cut;
 }
 
-// Rows with top-k up to CAP / 4: true if the draw was made.  `mine`: the thread's own maximum.
+// Rows with top-k up to CAP / 4: true if the draw was made.  `mine`, `mine2`: the thread's own two largest.
 template <typename T, int THREADS>
-__device__ __forceinline__ bool draw_from_first_k(Shared<THREADS>& s, const SampleArgs& a, int64_t r, const T* row, float top, float mine, const Rule& rule) {
+__device__ __forceinline__ bool draw_from_first_k(Shared<THREADS>& s, const SampleArgs& a, int64_t r, const T* row, float top, float mine, float mine2, const Rule& rule) {
     constexpr int BINS = Dim<THREADS>::BINS, CAP = Dim<THREADS>::CAP, PER = CAP / THREADS;
     const int32_t V = a.V;
     for (int b = threadIdx.x; b < BINS; b += THREADS) { s.count[b] = 0; s.mass[b] = 0; }
     if (threadIdx.x == 0) { s.n = 0; s.found = BINS; }
     __syncthreads();
     if (mine > -HUGE_VALF) atomicAdd(&s.count[bin_of<THREADS>(scaled(mine, top, rule.inv_t))], 1u);
+    if (mine2 > -HUGE_VALF) atomicAdd(&s.count[bin_of<THREADS>(scaled(mine2, top, rule.inv_t))], 1u);
     __syncthreads();
-    {   // the bin of the k-th largest thread maximum
+    {   // the bin of the k-th largest of those
         u64 n = 0, all;
 #pragma unroll
         for (int i = 0; i < BINS / THREADS; ++i) n += s.count[threadIdx.x * (BINS / THREADS) + i];
@@ -686,7 +691,7 @@ __device__ __forceinline__ bool draw_from_first_k(Shared<THREADS>& s, const Samp
     }
     __syncthreads();
     const uint32_t bin = s.found;
-    if (bin >= BINS - 1) return false;              // fewer than k maxima, or in the last bin, which has no lower edge
+    if (bin >= BINS - 1) return false;              // fewer than k of them, or in the last bin, which has no lower edge
     // no element of bins 0 .. bin lies below this
     const float limit = lower_edge<THREADS>(bin, top, rule.inv_t);
     each<T, THREADS>(row, V, [&](int32_t i, float l) {
@@ -766,7 +771,7 @@ __device__ __forceinline__ bool draw_from_first_k(Shared<THREADS>& s, const Samp
 }
 
 template <typename T, int THREADS>
-__global__ __launch_bounds__(THREADS) void sample_row_kernel(const SampleArgs a) {
+__global__ __launch_bounds__(THREADS, THREADS == 256 ? 6 : 4) void sample_row_kernel(const SampleArgs a) {
     __shared__ Shared<THREADS> s;
     constexpr int CE = Chunk<T>::n;
     const int64_t r = blockIdx.x;
@@ -776,8 +781,8 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(const SampleArgs a)
     const Rule rule = rule_of(a, r);
     if (threadIdx.x < 64) s.pow64[threadIdx.x] = kPow64[threadIdx.x];
     // maximum
-    float mine = -HUGE_VALF;
-    each<T, THREADS>(row, V, [&](int32_t, float l) { mine = fmaxf(mine, l); });
+    float mine = -HUGE_VALF, mine2 = -HUGE_VALF;
+    each<T, THREADS>(row, V, [&](int32_t, float l) { mine2 = fmaxf(mine2, fminf(mine, l)); mine = fmaxf(mine, l); });
     float top = mine;
 #pragma unroll
     for (int o = 32; o > 0; o /= 2) top = fmaxf(top, __shfl_xor(top, o));
@@ -801,7 +806,7 @@ __global__ __launch_bounds__(THREADS) void sample_row_kernel(const SampleArgs a)
         return;
     }
     if (rule.k > 0 && rule.k <= Dim<THREADS>::CAP / 4 && fabsf(top) < HUGE_VALF) {
-        if (draw_from_first_k<T, THREADS>(s, a, r, row, top, mine, rule)) return;
+        if (draw_from_first_k<T, THREADS>(s, a, r, row, top, mine, mine2, rule)) return;
         __syncthreads();
     }
     const Cut cut = rule.k > 0 || rule.p < 1.0 ? cut_of<T, THREADS>(s, row, V, top, rule) : Cut{0, 0xFFFFFFFFu};
@@ -913,7 +918,7 @@ template <typename T> void launch(const SampleArgs& a, hipStream_t stream) {
     else if (a.V <= 512) MARL_WAVE(8);
     else if (a.V <= 1024) MARL_WAVE(16);
     else if (a.V <= 2048) MARL_WAVE(32);
-    else if (a.V <= 8192) hipLaunchKernelGGL((sample_row_kernel<T, 256>), dim3((unsigned)a.rows), dim3(256), 0, stream, a);
+    else if (a.V <= 8192 || (a.rows >= 512 && a.V <= 131072)) hipLaunchKernelGGL((sample_row_kernel<T, 256>), dim3((unsigned)a.rows), dim3(256), 0, stream, a);
     else hipLaunchKernelGGL((sample_row_kernel<T, 1024>), dim3((unsigned)a.rows), dim3(1024), 0, stream, a);
 #undef MARL_SHORT
 #undef MARL_WAVE
