@@ -594,7 +594,7 @@ __global__ __launch_bounds__(256) void gated_finish_kernel(const ProductArgs arg
 }
 
 // da = gy p and, `half` columns behind it, db = gy f of every row, both padded with zeros: bandwidth (three reads, two writes of T h)
-template <typename T>
+template <typename T, bool WHOLE>
 __global__ __launch_bounds__(256) void gated_da_db_kernel(const T* __restrict__ f, const T* __restrict__ p, const T* __restrict__ gy, int64_t ldgy,
                                                            T* __restrict__ dab, int64_t half, int64_t rows, int64_t h) {
     constexpr int CE = Chunk<T>::n;
@@ -602,7 +602,8 @@ __global__ __launch_bounds__(256) void gated_da_db_kernel(const T* __restrict__ 
     for (int64_t t = blockIdx.y; t < rows; t += gridDim.y)
         for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < per; q += (int64_t)gridDim.x * 256) {
             const int64_t c = q * CE;
-            const Vec<T> vf = load_clipped(f + t * h, c, h), vp = load_clipped(p + t * h, c, h), vg = load_clipped(gy + t * ldgy, c, h);
+            auto load = [&](const T* row) { return WHOLE ? load_chunk(row + c) : load_clipped(row, c, h); };
+            const Vec<T> vf = load(f + t * h), vp = load(p + t * h), vg = load(gy + t * ldgy);
             Vec<T> da, db;
 #pragma unroll
             for (int i = 0; i < CE; ++i) {
@@ -619,14 +620,16 @@ __global__ __launch_bounds__(256) void gated_da_db_kernel(const T* __restrict__ 
 struct Plan { bool big; int slices, stages; };
 
 // Tile and split of one product.  256 x 256 tiles (one block of eight waves per CU) where they fill the chip, else
-// 128 x 128 (two blocks per CU); if those do not fill it either, k is cut into slices of at least sixteen stages.
+// 128 x 128; if those are too few for that, k is cut into slices of at least sixteen stages, up to one block for every CU.
+// Two blocks for every CU cost more in the slices' sum than they save (kernel and sum, one : two blocks a CU; T 1999,
+// d 1000, h 2731, float16, dx and dW: 89 : 95 us; T 32768, d 128, h 512, float32, dW: 93 : 102 us).
 template <typename T> Plan plan_of(int mode, int64_t M, int64_t N, int64_t K) {
     const int cus = marl_net::device_cus(256);
     const int64_t bk = ROW_BYTES / sizeof(T), all = (K + bk - 1) / bk * (mode == DX ? 2 : 1);
     auto tiles = [&](int64_t b) { return ((M + b - 1) / b) * ((N + b - 1) / b); };
     Plan p = {tiles(256) >= cus * 3 / 4, 1, (int)all};
     if (mode != FWD && !p.big) {
-        const int64_t want = 2 * cus / tiles(128), most = all / 16;
+        const int64_t want = cus / tiles(128), most = all / 16;
         const int64_t slices = want < 1 ? 1 : want < most ? want : most < 1 ? 1 : most;
         p.stages = (int)((all + slices - 1) / slices);
         p.slices = (int)((all + p.stages - 1) / p.stages);
@@ -753,7 +756,8 @@ template <typename T> int backward(Gated g, const void* f, const void* p, const 
     const int64_t half = packed_ld<T>(g.h), per = half / Chunk<T>::n;
     T* dab = (T*)ws;
     ws += round_256(g.rows * 2 * half * (int64_t)sizeof(T));
-    hipLaunchKernelGGL(gated_da_db_kernel<T>, dim3((unsigned)((per + 255) / 256), (unsigned)(g.rows < 65535 ? g.rows : 65535)), dim3(256), 0, stream,
+    auto* da_db = g.h % Chunk<T>::n == 0 ? gated_da_db_kernel<T, true> : gated_da_db_kernel<T, false>;
+    hipLaunchKernelGGL(da_db, dim3((unsigned)((per + 255) / 256), (unsigned)(g.rows < 65535 ? g.rows : 65535)), dim3(256), 0, stream,
                        (const T*)f, (const T*)p, (const T*)gy, ldgy, dab, half, g.rows, (int64_t)g.h);
     hipError_t err = hipGetLastError();
     if (err == hipSuccess && dx) {                // DX moves through both weights with one stride
