@@ -4,7 +4,8 @@
 // columns.  The gradient is the same function of gy, so a backward pass, a replayed rollout or a shuffled minibatch that
 // names its rows by the same keys meets the same mask.  A dropped element is 0 whatever it held.
 // Bandwidth bound (one read, one write) as long as the ~100 integer instructions of a call, a quarter of them 32-bit
-// multiplies, are shared by eight elements; with 32-bit draws (four a call) the generator would be the limit for 16-bit types.
+// multiplies, are shared by eight elements; 32-bit draws would take twice the calls.
+// Measured: 65536 x 512 float32 49 us (5.5 TB/s); 4099 x 1537 bf16 8.1 us (3.1 TB/s), 6.9 us a call without the profiler.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

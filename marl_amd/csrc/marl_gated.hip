@@ -16,6 +16,10 @@
 // 16-bit types: v_mfma_f32_32x32x16 with float32 accumulators; float32: v_mfma_f32_32x32x2.  da and db are rounded to
 // the element type, once, because they are matrix operands; f and p are kept in it between forward and backward (T h
 // elements each, against 4 T d h operations for computing a and b again).
+// Bound by the matrix cores; FWD / DX / DW measured: T 8192, d 2048, h 8192, bf16: 621 / 465 / 472 us (885 / 1183 / 1165
+// TFLOP/s); T 32768, d 128, h 512, float32: 105 / 80 / 77 us (82 / 108 / 111); T 1999, d 1000, h 2731, float16, operands
+// packed: 50 / 36 / 37 us (436 / 601 / 592).  da and db are bandwidth: 109 us at the first sizes (6.1 TB/s).  Few rows are
+// bound by the weights' bytes: T 1, d 2048, h 8192, bf16: 13.9 us a call (4.8 TB/s).
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>

@@ -17,6 +17,9 @@
 // the few elements above are sorted in LDS and the rest happens there.  Otherwise: maximum; counts and masses over bins
 // of a fraction of a nat below the maximum; the elements of the bin in which a border falls, sorted in LDS; the masses of
 // the kept.
+// Measured: 131072 x 4 float32 6.8 us; 256 x 131072 bf16 with settings per row 66 to 151 us, by whether some row's settings
+// miss the short way for a small top-k (67 MB would take 13): one row's chain of passes on one CU is the bound, as for one
+// row of 100003 (22 us).
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>

@@ -469,7 +469,7 @@ def sample_check(logits, u, t=1.0, k=0, p=1.0, m=0.0, settings=None):
         s = (f32(t), k, f32(p), f32(m)) if settings is None else (float(settings[r, 0]), int(settings[r, 1]), float(settings[r, 2]), float(settings[r, 3]))
         i, want = sample_oracle(logits[r].double().numpy(), float(u[r]), *s)
         assert int(index[r]) == i, (r, int(index[r]), i, s)
-        # weights are rounded to 2^-44 of the largest; the result to float32
+        # weights are held in units of 2^-42 of the largest, each off by half of one; the result is rounded to float32
         assert lp[r] == want if np.isinf(want) else abs(float(lp[r]) - want) <= U * abs(want) + V * 2.0 ** -43 + 1e-12, (r, float(lp[r]), want)
 
 
