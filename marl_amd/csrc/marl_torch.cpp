@@ -52,6 +52,14 @@ void same_type(const char* op, const Tensor& first, std::initializer_list<const 
     TORCH_CHECK_VALUE(t == at::kFloat || t == at::kBFloat16 || t == at::kHalf, op, ": float32, bfloat16 or float16 tensors, not ", t);
     for (const Tensor* r : rest) TORCH_CHECK_VALUE(!r || !r->defined() || r->scalar_type() == t, op, ": all of these tensors must be ", t);
 }
+// sizes that the C entry points take as 32 bits: refused here, before they are cut (the entry points have limits of their own)
+void fits_32(const char* op, std::initializer_list<int64_t> sizes) {
+    for (const int64_t n : sizes) TORCH_CHECK_VALUE(n <= INT32_MAX, op, ": rows of at most 2^31 - 1 elements, and as many weight rows");
+}
+// what forward kept for a backward pass: contiguous, of this shape
+void check_kept(const char* op, const Tensor& t, at::IntArrayRef sizes) {
+    TORCH_CHECK_VALUE(t.sizes() == sizes && t.is_contiguous(), op, ": tensors kept by forward must be contiguous ", sizes, ", not ", t.sizes());
+}
 // one HIP device
 void same_device(const char* op, const Tensor& first, std::initializer_list<const Tensor*> rest) {
     for (const Tensor* r : rest) TORCH_CHECK_VALUE(!r || !r->defined() || r->device() == first.device(), op, ": tensors on different devices");
@@ -121,6 +129,7 @@ std::vector<int64_t> check_gated(const Tensor& x, const Tensor& wg, const Tensor
     TORCH_CHECK_VALUE(wg.dim() == 2 && wu.sizes() == wg.sizes(), "gated_linear: w_gate and w_up must be [h, d] of one shape");
     TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) == wg.size(1), "gated_linear: x must be [..., d] for weights [h, d]");
     TORCH_CHECK_VALUE(wg.size(0) > 0 && wg.size(1) > 0, "gated_linear: weights without elements");
+    fits_32("gated_linear", {wg.size(0), wg.size(1)});
     same_type("gated_linear", x, {&wg, &wu});
     return with_last(x.sizes(), wg.size(0));
 }
@@ -146,7 +155,17 @@ Tensor3 gated_launch(const Tensor& x, const Tensor& wg, const Tensor& wu, c10::s
 Tensor gated_linear(const Tensor& x, const Tensor& wg, const Tensor& wu, c10::string_view act) { return std::get<0>(gated_launch(x, wg, wu, act, false)); }
 Tensor3 gated_linear_saved(const Tensor& x, const Tensor& wg, const Tensor& wu, c10::string_view act) { return gated_launch(x, wg, wu, act, true); }
 
+void check_gated_backward(const Tensor& gy, const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& f, const Tensor& p) {
+    const auto shape = check_gated(x, wg, wu, "silu");
+    TORCH_CHECK_VALUE(gy.sizes() == at::IntArrayRef(shape), "gated_linear: gy must be shaped like the result");
+    check_kept("gated_linear", f, shape);
+    check_kept("gated_linear", p, shape);
+    same_type("gated_linear", x, {&gy, &f, &p});
+}
+
 Tensor3 gated_linear_backward(const Tensor& gy, const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& f, const Tensor& p, bool need_x, bool need_w) {
+    check_gated_backward(gy, x, wg, wu, f, p);
+    same_device("gated_linear", x, {&gy, &wg, &wu, &f, &p});
     const int64_t h = wg.size(0), d = wg.size(1);
     Tensor dx = need_x ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options());
     Tensor dg = need_w ? at::empty({h, d}, x.options()) : at::empty({0}, x.options()), du = at::empty_like(dg);
@@ -166,7 +185,8 @@ Tensor gated_linear_meta(const Tensor& x, const Tensor& wg, const Tensor& wu, c1
 Tensor3 gated_linear_saved_meta(const Tensor& x, const Tensor& wg, const Tensor& wu, c10::string_view act) {
     return {gated_linear_meta(x, wg, wu, act), gated_linear_meta(x, wg, wu, act), gated_linear_meta(x, wg, wu, act)};
 }
-Tensor3 gated_linear_backward_meta(const Tensor&, const Tensor& x, const Tensor& wg, const Tensor&, const Tensor&, const Tensor&, bool need_x, bool need_w) {
+Tensor3 gated_linear_backward_meta(const Tensor& gy, const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& f, const Tensor& p, bool need_x, bool need_w) {
+    check_gated_backward(gy, x, wg, wu, f, p);
     const auto w = [&] { return need_w ? at::empty(wg.sizes(), x.options()) : at::empty({0}, x.options()); };
     return {need_x ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options()), w(), w()};
 }
@@ -247,8 +267,21 @@ Tensor3 residual_norm_saved(const Tensor& x, const Tensor& block, const Tensor& 
     return norm_launch(x, block, wpost, wpre, gate, scale, eps, kind, true);
 }
 
+void check_norm_backward(const optional<Tensor>& gy, const optional<Tensor>& gn, const Tensor& y, const Tensor& block, const Tensor& wpost,
+                         const Tensor& wpre, const optional<Tensor>& gate, const Tensor& stats, c10::string_view kind) {
+    check_norm(y, block, wpost, wpre, gate, 0.0, kind);
+    for (const Tensor* g : {ptr(gy), ptr(gn)})
+        TORCH_CHECK_VALUE(!g || !g->defined() || g->sizes() == y.sizes(), "residual_norm: gy and gn must be shaped like the results");
+    check_kept("residual_norm", y, y.sizes());
+    check_kept("residual_norm", stats, with_last(y.sizes(), 4));
+    TORCH_CHECK_VALUE(stats.scalar_type() == at::kFloat, "residual_norm: stats must be float32");
+    same_type("residual_norm", y, {ptr(gy), ptr(gn)});
+}
+
 Tensor5 residual_norm_backward(const optional<Tensor>& gy, const optional<Tensor>& gn, const Tensor& y, const Tensor& block, const Tensor& wpost,
                                const Tensor& wpre, const optional<Tensor>& gate, const Tensor& stats, double scale, c10::string_view kind) {
+    check_norm_backward(gy, gn, y, block, wpost, wpre, gate, stats, kind);
+    same_device("residual_norm", y, {ptr(gy), ptr(gn), &block, &wpost, &wpre, ptr(gate), &stats});
     const int64_t d = y.size(-1);
     Tensor dx = at::empty(y.sizes(), y.options()), db = at::empty(y.sizes(), y.options()), dpost = at::empty({d}, y.options()), dpre = at::empty({d}, y.options());
     Tensor dgate = gate ? at::empty(gate->sizes(), y.options()) : at::empty({0}, y.options());
@@ -277,8 +310,9 @@ Tensor3 residual_norm_saved_meta(const Tensor& x, const Tensor& block, const Ten
     auto [y, n] = residual_norm_meta(x, block, wpost, wpre, gate, scale, eps, kind);
     return {y, n, at::empty(with_last(x.sizes(), 4), x.options().dtype(at::kFloat))};
 }
-Tensor5 residual_norm_backward_meta(const optional<Tensor>&, const optional<Tensor>&, const Tensor& y, const Tensor&, const Tensor& wpost, const Tensor&,
-                                    const optional<Tensor>& gate, const Tensor&, double, c10::string_view) {
+Tensor5 residual_norm_backward_meta(const optional<Tensor>& gy, const optional<Tensor>& gn, const Tensor& y, const Tensor& block, const Tensor& wpost, const Tensor& wpre,
+                                    const optional<Tensor>& gate, const Tensor& stats, double, c10::string_view kind) {
+    check_norm_backward(gy, gn, y, block, wpost, wpre, gate, stats, kind);
     return {at::empty(y.sizes(), y.options()), at::empty(y.sizes(), y.options()), at::empty(wpost.sizes(), y.options()), at::empty(wpost.sizes(), y.options()),
             gate ? at::empty(gate->sizes(), y.options()) : at::empty({0}, y.options())};
 }
@@ -322,6 +356,7 @@ void check_dropout(const Tensor& x, double p, const optional<Tensor>& keys) {
     TORCH_CHECK_VALUE(!keys || (keys->scalar_type() == at::kLong && keys->sizes() == x.sizes().slice(0, x.dim() - 1)),
                       "keyed_dropout: keys must be int64, one per row of x");
     same_type("keyed_dropout", x, {});
+    fits_32("keyed_dropout", {x.size(-1)});
 }
 Tensor keyed_dropout(const Tensor& x, double p, int64_t seed, const optional<Tensor>& keys) {
     check_dropout(x, p, keys);

@@ -109,3 +109,59 @@ def test_gated_trunk_is_refused_on_the_cpu_and_the_default_networks_are_unchange
     assert [k for k in Actor().state_dict()][:2] == ["trunk.0.weight", "trunk.0.bias"] and "network.4.bias" in Critic().state_dict()
     agent = PPOAgent(device="cpu", seed=1)
     assert set(agent._config()) & {"trunk", "trunk_blocks", "trunk_dropout"} == set()
+
+
+def M(*shape, dtype=torch.float32):
+    return torch.empty(*shape, dtype=dtype, device="meta")
+
+
+# x [2, 3], weights [4, 3], what forward keeps [2, 4]
+GATED = dict(gy=(2, 4), x=(2, 3), w_gate=(4, 3), w_up=(4, 3), f=(2, 4), p=(2, 4))
+NORM = dict(gy=(2, 3), gn=(2, 3), y=(2, 3), block=(2, 3), w_post=(3,), w_pre=(3,), gate=(3,), stats=(2, 4))
+
+
+def gated_backward(**other):
+    t = {k: M(*s) for k, s in GATED.items()}
+    t.update(other)
+    return ops.gated_linear_backward(*t.values(), True, True)
+
+
+def norm_backward(**other):
+    t = {k: M(*s) for k, s in NORM.items()}
+    t.update(other)
+    return ops.residual_norm_backward(*t.values(), 1.0, "rms")
+
+
+def test_backward_shapes():
+    assert [tuple(g.shape) for g in gated_backward()] == [(2, 3), (4, 3), (4, 3)]
+    assert [tuple(g.shape) for g in norm_backward()] == [(2, 3), (2, 3), (3,), (3,), (3,)]
+    assert len(norm_backward(gy=None, gate=None)) == 5
+
+
+@pytest.mark.parametrize("name", ["gy", "f", "p"])
+def test_gated_backward_refuses_what_forward_did_not_keep(name):
+    bad = [M(1, 4), M(2, 3), M(2, 4, dtype=torch.float16)] + ([] if name == "gy" else [M(4, 2).t()])
+    for t in bad:
+        with pytest.raises(ValueError):
+            gated_backward(**{name: t})
+
+
+@pytest.mark.parametrize("name", ["gy", "gn", "y", "block", "w_post", "w_pre", "gate", "stats"])
+def test_norm_backward_refuses_what_forward_did_not_keep(name):
+    bad = [M(1, 3), M(2, 2), M(*NORM[name], dtype=torch.float16)] + ([M(3, 2).t()] if name == "y" else [M(4, 2).t()] if name == "stats" else [])
+    for t in bad:
+        with pytest.raises(ValueError):
+            norm_backward(**{name: t})
+
+
+BEYOND = (1 << 32) + 1          # cut to 32 bits this is 1
+
+
+@pytest.mark.parametrize("call", [
+    lambda: ops.gated_linear(M(1, 1), M(BEYOND, 1), M(BEYOND, 1)),
+    lambda: ops.gated_linear(M(1, BEYOND), M(1, BEYOND), M(1, BEYOND)),
+    lambda: ops.keyed_dropout(M(1, BEYOND), 0.5, 1),
+])
+def test_sizes_beyond_32_bits_are_refused(call):
+    with pytest.raises(ValueError):
+        call()
