@@ -703,3 +703,34 @@ def test_results_do_not_vary_from_run_to_run():
     first = once()
     for _ in range(3):
         assert all(torch.equal(p, q) for p, q in zip(first, once()))
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.float16], ids=str)
+def test_sample_logits_many_long_rows(dt):
+    # many rows above 8192 logits take smaller workgroups than a few: the draws are those of the definition, and a row drawn
+    # among many is the row drawn among few, bit for bit (integer weights), on both sides of the limits of top-k
+    R, V = 516, 8203
+    g = torch.Generator().manual_seed(11)
+    logits = (3 * torch.randn(R, V, generator=g)).to(dt)
+    logits[torch.rand(R, V, generator=g) < 0.1] = float("-inf")
+    logits[5] = 1.0                                    # one value
+    logits[6] = float("-inf")                          # nothing
+    logits[7, 2:] = float("-inf")                      # fewer than k
+    logits[8, 4000:4300] = 20.0                        # ties across every limit below
+    logits[9, 77] = float("inf")
+    u = torch.rand(R, generator=g)
+    ks = torch.tensor([0, 1, 64, 255, 256, 257, 511, 512, 513, 1025])
+    settings = torch.stack([0.5 + torch.rand(R, generator=g), ks[torch.arange(R) % len(ks)].float(), torch.where(torch.rand(R, generator=g) < 0.5, 0.9, 1.0),
+                            torch.where(torch.rand(R, generator=g) < 0.3, 0.01, 0.0)], 1).contiguous()
+    dev = [t.cuda() for t in (logits, u, settings)]
+    many = ops.sample_logits(dev[0], dev[1], settings=dev[2])
+    for first in range(0, R, 129):
+        s = slice(first, first + 129)
+        few = ops.sample_logits(dev[0][s], dev[1][s], settings=dev[2][s])
+        assert torch.equal(many[0][s], few[0]) and torch.equal(many[1][s], few[1])
+    pick = torch.cat([torch.arange(0, 40), torch.arange(40, R, 7)])
+    index, lp = many[0].cpu(), many[1].cpu()
+    for r in pick.tolist():
+        i, want = sample_oracle(logits[r].double().numpy(), float(u[r]), float(settings[r, 0]), int(settings[r, 1]), float(settings[r, 2]), float(settings[r, 3]))
+        assert int(index[r]) == i, (r, int(index[r]), i, settings[r])
+        assert float(lp[r]) == want if np.isinf(want) else abs(float(lp[r]) - want) <= U * abs(want) + V * 2.0 ** -43 + 1e-12, (r, float(lp[r]), want)
