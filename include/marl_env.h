@@ -502,10 +502,10 @@ int marl_gated_backward(int32_t dtype, int64_t rows, int32_t d, int32_t h, const
 int marl_residual_norm(int32_t dtype, int32_t kind, int64_t rows, int32_t d, const void *x, int64_t ldx, const void *block,
                        int64_t ld_block, const void *w_post, const void *w_pre, const void *gate, int64_t ld_gate,
                        float scale, float eps, void *y, void *n, float *stats, void *stream);
-/* Gradients from gy and gn (either may be NULL: zero): dx, dblock [rows][d], dw_post, dw_pre [d], dgate (shaped like gate,
- * given exactly when gate is), all contiguous.  workspace: 16-byte aligned, marl_residual_norm_workspace_bytes. */
+/* Gradients from gy and gn (either may be NULL: zero) and the x [rows][d], contiguous, of the forward call: dx, dblock
+ * [rows][d], dw_post, dw_pre [d], dgate (shaped like gate, given exactly when gate is), all contiguous.  workspace: 16-byte aligned, marl_residual_norm_workspace_bytes. */
 size_t marl_residual_norm_workspace_bytes(int32_t d);
-int marl_residual_norm_backward(int32_t dtype, int32_t kind, int64_t rows, int32_t d, const void *y, const void *block,
+int marl_residual_norm_backward(int32_t dtype, int32_t kind, int64_t rows, int32_t d, const void *x, const void *block,
                                 int64_t ld_block, const void *w_post, const void *w_pre, const void *gate, int64_t ld_gate,
                                 const float *stats, const void *gy, int64_t ld_gy, const void *gn, int64_t ld_gn, float scale,
                                 void *dx, void *dblock, void *dw_post, void *dw_pre, void *dgate, void *workspace, void *stream);

@@ -5,11 +5,12 @@
 //     dx = scale t,  dgate = t o,  dblock = N'(t gate w_post; block),  dw_post = sum t gate block^,  dw_pre = sum gn y^,
 //     N'(g; v) = r (g - mean(g) [layer only] - v^ mean(g v^)).
 // Bandwidth bound: a row lives in the registers of its threads (16 lanes to 1024 threads, one 16-byte chunk each as long as
-// that is enough), so that forward reads x and block once and backward gy, gn, y and block once.  Workgroups stay and take
+// that is enough), so that forward reads x and block once and backward gy, gn, x and block once.  Workgroups stay and take
 // row after row: the next row's chunks are under way while the sums of this one cross the waves, and the weights' chunks
 // are held throughout.  Sums and statistics are float32; y is
-// normalised before it is rounded.  m and r of both norms are kept (16 bytes a row) so that backward uses the unrounded
-// rows' statistics.  The column sums of backward stay in registers over a workgroup's rows, go to a partial row per
+// normalised before it is rounded.  m and r of both norms are kept (16 bytes a row), and backward computes y from x and block
+// again: taken from memory, y has been rounded, and with the statistics of the unrounded row that leaves an error of half a
+// step of y, times r, in y^ (a row of mean 64 and spread 1 in bf16: 0.14), at the same bytes.  The column sums of backward stay in registers over a workgroup's rows, go to a partial row per
 // workgroup and are added by a second launch in a fixed order (no atomics: results do not vary from run to run).
 // Measured: forward 131072 x 128 float32 43 us (6.2 TB/s), 16384 x 4096 bf16 100 us (5.4); backward there 220 us (3.7), where
 // the column partials take the registers that more rows under way would need, and 7 us for their sum.
@@ -208,7 +209,8 @@ __device__ __forceinline__ void norm_back(Regs<T, NV>& g, const Regs<T, NV>& h, 
     FOR_ROW(i, e) g.v[i][e] = r * (g.v[i][e] - s - h.v[i][e] * p);
 }
 
-template <typename T, int NV, int LANES, int WIDTH>
+// GATE is known at compile time: without a channel gate its column sums take no registers, without any gate neither its chunks.
+template <typename T, int NV, int LANES, int WIDTH, int GATE>
 __global__ __launch_bounds__(Row<LANES>::THREADS) void residual_norm_backward_kernel(const NormArgs a) {
     using R = Row<LANES>;
     constexpr int CE = Chunk<T>::n;
@@ -218,18 +220,19 @@ __global__ __launch_bounds__(Row<LANES>::THREADS) void residual_norm_backward_ke
     const int lane = threadIdx.x % LANES, slot = threadIdx.x / LANES;
     const int32_t d = a.d;
     Regs<T, NV> spost = {}, spre = {}, sgate = {};
-    P wpost, wpre, gate, ny, ngn, ngy, nb;
+    P wpost, wpre, gate, nx, ngn, ngy, nb, ngate;
     float4 nst;
     load_row<T, NV, LANES, WIDTH>(wpost, (const T*)a.w_post, d, lane);
     load_row<T, NV, LANES, WIDTH>(wpre, (const T*)a.w_pre, d, lane);
-    if (a.gate_kind == CHANNEL_GATE) load_row<T, NV, LANES, WIDTH>(gate, (const T*)a.gate, d, lane);
+    if constexpr (GATE == CHANNEL_GATE) load_row<T, NV, LANES, WIDTH>(gate, (const T*)a.gate, d, lane);
     auto fetch = [&](int64_t r0) {
         const int64_t r = r0 + slot < a.rows ? r0 + slot : a.rows - 1;
         nst = *(const float4*)(a.stats + 4 * r);
-        load_row<T, NV, LANES, WIDTH>(ny, (const T*)a.y + r * d, d, lane);
+        load_row<T, NV, LANES, WIDTH>(nx, (const T*)a.x + r * a.ldx, d, lane);
         load_row<T, NV, LANES, WIDTH>(nb, (const T*)a.block + r * a.ldb, d, lane);
         if (a.gn) load_row<T, NV, LANES, WIDTH>(ngn, (const T*)a.gn + r * a.ldgn, d, lane);
         if (a.gy) load_row<T, NV, LANES, WIDTH>(ngy, (const T*)a.gy + r * a.ldgy, d, lane);
+        if constexpr (GATE == ROW_GATE) load_row<T, NV, LANES, WIDTH>(ngate, (const T*)a.gate + r * a.ldg, d, lane);
     };
     const int64_t turn = (int64_t)gridDim.x * R::ROWS;
     int64_t r0 = (int64_t)blockIdx.x * R::ROWS;
@@ -239,12 +242,25 @@ __global__ __launch_bounds__(Row<LANES>::THREADS) void residual_norm_backward_ke
         const int64_t r = live ? r0 + slot : a.rows - 1;
         const float4 st = nst;
         const P gy = ngy, block = nb;
+        if constexpr (GATE == ROW_GATE) gate = ngate;
         auto there = [&](int i, int e) { return live && (i * LANES + lane) * CE + e < d; };
         Regs<T, NV> h, t;
         float w[CE], g[CE];
+        // y as forward had it before rounding: the statistics are of that one
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            unpack<T, NV, LANES, WIDTH>(h.v[i], ny, i, d, lane);
+            unpack<T, NV, LANES, WIDTH>(h.v[i], block, i, d, lane);
+            unpack<T, NV, LANES, WIDTH>(w, wpost, i, d, lane);
+#pragma unroll
+            for (int e = 0; e < CE; ++e) h.v[i][e] = (h.v[i][e] - st.x) * st.y * w[e];
+            if constexpr (GATE != NO_GATE) {
+                unpack<T, NV, LANES, WIDTH>(g, gate, i, d, lane);
+#pragma unroll
+                for (int e = 0; e < CE; ++e) h.v[i][e] *= g[e];
+            }
+            unpack<T, NV, LANES, WIDTH>(w, nx, i, d, lane);
+#pragma unroll
+            for (int e = 0; e < CE; ++e) h.v[i][e] = fmaf(a.scale, w[e], h.v[i][e]);
             unpack<T, NV, LANES, WIDTH>(g, ngn, i, d, lane, live && a.gn);
             unpack<T, NV, LANES, WIDTH>(w, wpre, i, d, lane);
 #pragma unroll
@@ -254,7 +270,6 @@ __global__ __launch_bounds__(Row<LANES>::THREADS) void residual_norm_backward_ke
                 t.v[i][e] = g[e] * w[e];
             }
         }
-        if (a.gate_kind == ROW_GATE) load_row<T, NV, LANES, WIDTH>(gate, (const T*)a.gate + r * a.ldg, d, lane);
         if (r0 + turn < a.rows) fetch(r0 + turn);
         norm_back<T, NV, LANES>(t, h, d, a.layer, st.w, scratch);
 #pragma unroll
@@ -272,20 +287,20 @@ __global__ __launch_bounds__(Row<LANES>::THREADS) void residual_norm_backward_ke
         for (int i = 0; i < NV; ++i) {
             unpack<T, NV, LANES, WIDTH>(h.v[i], block, i, d, lane);
             unpack<T, NV, LANES, WIDTH>(w, wpost, i, d, lane);
-            if (a.gate_kind != NO_GATE) unpack<T, NV, LANES, WIDTH>(g, gate, i, d, lane);
+            if constexpr (GATE != NO_GATE) unpack<T, NV, LANES, WIDTH>(g, gate, i, d, lane);
 #pragma unroll
             for (int e = 0; e < CE; ++e) {
                 h.v[i][e] = there(i, e) ? (h.v[i][e] - st.x) * st.y : 0.0f;
-                if (a.gate_kind != NO_GATE) {
+                if constexpr (GATE != NO_GATE) {
                     dg.v[i][e] = t.v[i][e] * h.v[i][e] * w[e];
-                    if (live) sgate.v[i][e] += dg.v[i][e];
+                    if (GATE == CHANNEL_GATE && live) sgate.v[i][e] += dg.v[i][e];
                     t.v[i][e] *= g[e];
                 }
                 if (live) spost.v[i][e] = fmaf(t.v[i][e], h.v[i][e], spost.v[i][e]);
                 t.v[i][e] *= w[e];
             }
         }
-        if (a.gate_kind == ROW_GATE) store_row<T, NV, LANES>((T*)a.dgate_rows + r * d, dg, d, lane, live);
+        if constexpr (GATE == ROW_GATE) store_row<T, NV, LANES>((T*)a.dgate_rows + r * d, dg, d, lane, live);
         norm_back<T, NV, LANES>(t, h, d, a.layer, st.y, scratch);
         store_row<T, NV, LANES>((T*)a.dblock + r * d, t, d, lane, live);
     }
@@ -308,7 +323,7 @@ __global__ __launch_bounds__(Row<LANES>::THREADS) void residual_norm_backward_ke
     };
     put(0, spost);
     put(1, spre);
-    if (a.gate_kind == CHANNEL_GATE) put(2, sgate);
+    if constexpr (GATE == CHANNEL_GATE) put(2, sgate);
 }
 
 // dw_post, dw_pre, dgate: the partial rows added in a fixed order.  64 columns per workgroup, every 16th row per wave.
@@ -380,7 +395,10 @@ template <typename T> int backward(const NormArgs& a, void* dw_post, void* dw_pr
         // four turns or more a workgroup, so that adding the partial rows stays cheap, but one for every CU if there are rows
         const int64_t turns = (a.rows + R::ROWS - 1) / R::ROWS, want = turns / 4 > 256 ? turns / 4 : turns < 256 ? turns : 256;
         blocks = (int)(want < max_blocks(a.d) ? want : max_blocks(a.d));
-        hipLaunchKernelGGL((residual_norm_backward_kernel<T, NV, LANES, WIDTH>), dim3(blocks), dim3(R::THREADS), 0, stream, a);
+        auto* kernel = a.gate_kind == NO_GATE        ? residual_norm_backward_kernel<T, NV, LANES, WIDTH, NO_GATE>
+                       : a.gate_kind == CHANNEL_GATE ? residual_norm_backward_kernel<T, NV, LANES, WIDTH, CHANNEL_GATE>
+                                                     : residual_norm_backward_kernel<T, NV, LANES, WIDTH, ROW_GATE>;
+        hipLaunchKernelGGL(kernel, dim3(blocks), dim3(R::THREADS), 0, stream, a);
         return hipGetLastError();
     });
     if (err == hipSuccess) {
@@ -422,19 +440,19 @@ size_t marl_residual_norm_workspace_bytes(int32_t d) {
     return d < 1 || d > MARL_MAX_NORM_WIDTH ? 0 : (size_t)max_blocks(d) * 3 * d * sizeof(float);
 }
 
-int marl_residual_norm_backward(int32_t dtype, int32_t kind, int64_t rows, int32_t d, const void* y, const void* block, int64_t ld_block,
+int marl_residual_norm_backward(int32_t dtype, int32_t kind, int64_t rows, int32_t d, const void* x, const void* block, int64_t ld_block,
                                 const void* w_post, const void* w_pre, const void* gate, int64_t ld_gate, const float* stats, const void* gy,
                                 int64_t ld_gy, const void* gn, int64_t ld_gn, float scale, void* dx, void* dblock, void* dw_post,
                                 void* dw_pre, void* dgate, void* workspace, void* stream) {
     const int rc = check_sizes(dtype, kind, rows, d);
     if (rc != MARL_OK) return rc;
-    if (!y || !block || !w_post || !w_pre || !stats || !dx || !dblock || !dw_post || !dw_pre || !workspace || (gate == nullptr) != (dgate == nullptr) ||
+    if (!x || !block || !w_post || !w_pre || !stats || !dx || !dblock || !dw_post || !dw_pre || !workspace || (gate == nullptr) != (dgate == nullptr) ||
         ((uintptr_t)stats & 15) || ((uintptr_t)workspace & 15)) return MARL_EINVAL;
     if (rows > 1 && (ld_block < d || (gy && ld_gy < d) || (gn && ld_gn < d) || (gate && ld_gate != 0 && ld_gate < d))) return MARL_EINVAL;
     NormArgs a = {};
     a.block = block; a.w_post = w_post; a.w_pre = w_pre; a.gate = gate;
-    a.ldb = ld_block; a.ldg = ld_gate;
-    a.y = const_cast<void*>(y); a.stats = const_cast<float*>(stats);
+    a.x = x; a.ldx = d; a.ldb = ld_block; a.ldg = ld_gate;
+    a.stats = const_cast<float*>(stats);
     a.gy = gy; a.gn = gn; a.ldgy = ld_gy; a.ldgn = ld_gn;
     a.dx = dx; a.dblock = dblock; a.dgate_rows = dgate; a.partial = (float*)workspace;
     a.rows = rows; a.d = d;

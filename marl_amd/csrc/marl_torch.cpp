@@ -267,34 +267,35 @@ Tensor3 residual_norm_saved(const Tensor& x, const Tensor& block, const Tensor& 
     return norm_launch(x, block, wpost, wpre, gate, scale, eps, kind, true);
 }
 
-void check_norm_backward(const optional<Tensor>& gy, const optional<Tensor>& gn, const Tensor& y, const Tensor& block, const Tensor& wpost,
+// x: contiguous, as the entry point takes it
+void check_norm_backward(const optional<Tensor>& gy, const optional<Tensor>& gn, const Tensor& x, const Tensor& block, const Tensor& wpost,
                          const Tensor& wpre, const optional<Tensor>& gate, const Tensor& stats, c10::string_view kind) {
-    check_norm(y, block, wpost, wpre, gate, 0.0, kind);
+    check_norm(x, block, wpost, wpre, gate, 0.0, kind);
     for (const Tensor* g : {ptr(gy), ptr(gn)})
-        TORCH_CHECK_VALUE(!g || !g->defined() || g->sizes() == y.sizes(), "residual_norm: gy and gn must be shaped like the results");
-    check_kept("residual_norm", y, y.sizes());
-    check_kept("residual_norm", stats, with_last(y.sizes(), 4));
+        TORCH_CHECK_VALUE(!g || !g->defined() || g->sizes() == x.sizes(), "residual_norm: gy and gn must be shaped like the results");
+    check_kept("residual_norm", x, x.sizes());
+    check_kept("residual_norm", stats, with_last(x.sizes(), 4));
     TORCH_CHECK_VALUE(stats.scalar_type() == at::kFloat, "residual_norm: stats must be float32");
-    same_type("residual_norm", y, {ptr(gy), ptr(gn)});
+    same_type("residual_norm", x, {ptr(gy), ptr(gn)});
 }
 
-Tensor5 residual_norm_backward(const optional<Tensor>& gy, const optional<Tensor>& gn, const Tensor& y, const Tensor& block, const Tensor& wpost,
+Tensor5 residual_norm_backward(const optional<Tensor>& gy, const optional<Tensor>& gn, const Tensor& x, const Tensor& block, const Tensor& wpost,
                                const Tensor& wpre, const optional<Tensor>& gate, const Tensor& stats, double scale, c10::string_view kind) {
-    check_norm_backward(gy, gn, y, block, wpost, wpre, gate, stats, kind);
-    same_device("residual_norm", y, {ptr(gy), ptr(gn), &block, &wpost, &wpre, ptr(gate), &stats});
-    const int64_t d = y.size(-1);
-    Tensor dx = at::empty(y.sizes(), y.options()), db = at::empty(y.sizes(), y.options()), dpost = at::empty({d}, y.options()), dpre = at::empty({d}, y.options());
-    Tensor dgate = gate ? at::empty(gate->sizes(), y.options()) : at::empty({0}, y.options());
-    if (!y.numel()) return {dx, db, dpost.zero_(), dpre.zero_(), dgate.zero_()};
+    check_norm_backward(gy, gn, x, block, wpost, wpre, gate, stats, kind);
+    same_device("residual_norm", x, {ptr(gy), ptr(gn), &block, &wpost, &wpre, ptr(gate), &stats});
+    const int64_t d = x.size(-1);
+    Tensor dx = at::empty(x.sizes(), x.options()), db = at::empty(x.sizes(), x.options()), dpost = at::empty({d}, x.options()), dpre = at::empty({d}, x.options());
+    Tensor dgate = gate ? at::empty(gate->sizes(), x.options()) : at::empty({0}, x.options());
+    if (!x.numel()) return {dx, db, dpost.zero_(), dpre.zero_(), dgate.zero_()};
     const Rows rb(block);
-    const GateRows g(gate, y);
+    const GateRows g(gate, x);
     const Tensor wo = wpost.contiguous(), wr = wpre.contiguous();
     optional<Rows> ry, rn;
     if (gy && gy->defined()) ry.emplace(*gy);
     if (gn && gn->defined()) rn.emplace(*gn);
-    const On on(y);
-    Tensor ws = scratch(y, lib.marl_residual_norm_workspace_bytes((int32_t)d));
-    check(lib.marl_residual_norm_backward(type_code(y), kind_code(kind), rb.n, (int32_t)d, y.const_data_ptr(), rb.p(), rb.ld, wo.const_data_ptr(),
+    const On on(x);
+    Tensor ws = scratch(x, lib.marl_residual_norm_workspace_bytes((int32_t)d));
+    check(lib.marl_residual_norm_backward(type_code(x), kind_code(kind), rb.n, (int32_t)d, x.const_data_ptr(), rb.p(), rb.ld, wo.const_data_ptr(),
                                           wr.const_data_ptr(), g.p(), g.ld, stats.const_data_ptr<float>(), ry ? ry->p() : nullptr, ry ? ry->ld : 0,
                                           rn ? rn->p() : nullptr, rn ? rn->ld : 0, (float)scale, dx.mutable_data_ptr(), db.mutable_data_ptr(),
                                           dpost.mutable_data_ptr(), dpre.mutable_data_ptr(), gate ? dgate.mutable_data_ptr() : nullptr,
@@ -310,11 +311,11 @@ Tensor3 residual_norm_saved_meta(const Tensor& x, const Tensor& block, const Ten
     auto [y, n] = residual_norm_meta(x, block, wpost, wpre, gate, scale, eps, kind);
     return {y, n, at::empty(with_last(x.sizes(), 4), x.options().dtype(at::kFloat))};
 }
-Tensor5 residual_norm_backward_meta(const optional<Tensor>& gy, const optional<Tensor>& gn, const Tensor& y, const Tensor& block, const Tensor& wpost, const Tensor& wpre,
+Tensor5 residual_norm_backward_meta(const optional<Tensor>& gy, const optional<Tensor>& gn, const Tensor& x, const Tensor& block, const Tensor& wpost, const Tensor& wpre,
                                     const optional<Tensor>& gate, const Tensor& stats, double, c10::string_view kind) {
-    check_norm_backward(gy, gn, y, block, wpost, wpre, gate, stats, kind);
-    return {at::empty(y.sizes(), y.options()), at::empty(y.sizes(), y.options()), at::empty(wpost.sizes(), y.options()), at::empty(wpost.sizes(), y.options()),
-            gate ? at::empty(gate->sizes(), y.options()) : at::empty({0}, y.options())};
+    check_norm_backward(gy, gn, x, block, wpost, wpre, gate, stats, kind);
+    return {at::empty(x.sizes(), x.options()), at::empty(x.sizes(), x.options()), at::empty(wpost.sizes(), x.options()), at::empty(wpost.sizes(), x.options()),
+            gate ? at::empty(gate->sizes(), x.options()) : at::empty({0}, x.options())};
 }
 
 struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
@@ -322,7 +323,7 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         at::AutoDispatchBelowADInplaceOrView below;
         auto [y, n, stats] = handle<Tensor3(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const optional<Tensor>&, double, double, c10::string_view)>(
             "marl_amd::residual_norm_saved").call(x, block, wpost, wpre, gate, scale, eps, kind);
-        ctx->save_for_backward({y, block, wpost, wpre, gate ? *gate : Tensor(), stats});
+        ctx->save_for_backward({x, block, wpost, wpre, gate ? *gate : Tensor(), stats});
         ctx->saved_data["scale"] = scale;
         ctx->saved_data["kind"] = kind;
         ctx->set_materialize_grads(false);
@@ -334,7 +335,7 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         const auto given = [](const Tensor& t) { return t.defined() ? optional<Tensor>(t) : optional<Tensor>(); };
         auto [dx, db, dpost, dpre, dgate] = handle<Tensor5(const optional<Tensor>&, const optional<Tensor>&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
                                                            const optional<Tensor>&, const Tensor&, double, c10::string_view)>("marl_amd::residual_norm_backward")
-            .call(given(g[0]), given(g[1]), s[0], s[1], s[2], s[3], given(s[4]), s[5], ctx->saved_data["scale"].toDouble(), ctx->saved_data["kind"].toStringRef());
+            .call(given(g[0]), given(g[1]), s[0].contiguous(), s[1], s[2], s[3], given(s[4]), s[5], ctx->saved_data["scale"].toDouble(), ctx->saved_data["kind"].toStringRef());
         variable_list out = {dx, db, dpost, dpre, s[4].defined() ? dgate : Tensor(), Tensor(), Tensor(), Tensor()};
         for (size_t i = 0; i < (s[4].defined() ? 5 : 4); ++i) if (!ctx->needs_input_grad(i)) out[i] = Tensor();
         return once(std::move(out), "residual_norm");
@@ -459,7 +460,7 @@ TORCH_LIBRARY_FRAGMENT(marl_amd, m) {
     m.def("gated_linear_backward(Tensor gy, Tensor x, Tensor w_gate, Tensor w_up, Tensor f, Tensor p, bool need_x, bool need_w) -> (Tensor, Tensor, Tensor)");
     m.def("residual_norm(Tensor x, Tensor block, Tensor w_post, Tensor w_pre, Tensor? gate=None, float scale=1.0, float eps=1e-5, str kind=\"rms\") -> (Tensor, Tensor)");
     m.def("residual_norm_saved(Tensor x, Tensor block, Tensor w_post, Tensor w_pre, Tensor? gate, float scale, float eps, str kind) -> (Tensor, Tensor, Tensor)");
-    m.def("residual_norm_backward(Tensor? gy, Tensor? gn, Tensor y, Tensor block, Tensor w_post, Tensor w_pre, Tensor? gate, Tensor stats, float scale, str kind)"
+    m.def("residual_norm_backward(Tensor? gy, Tensor? gn, Tensor x, Tensor block, Tensor w_post, Tensor w_pre, Tensor? gate, Tensor stats, float scale, str kind)"
           " -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
     m.def("keyed_dropout(Tensor x, float p, int seed, Tensor? keys=None) -> Tensor");
     m.def("sample_logits(Tensor logits, Tensor u, float temperature=1.0, int top_k=0, float top_p=1.0, float min_p=0.0, *, Tensor? settings=None) -> (Tensor, Tensor)");
