@@ -481,11 +481,11 @@ enum { MARL_NORM_RMS = 0, MARL_NORM_LAYER = 1 };
 #define MARL_MAX_CHOICES (1 << 20)
 
 /* y[t][j] = act(a[t][j]) b[t][j],  a = x w_gate^T,  b = x w_up^T;  x [rows][d], weights [h][d], y [rows][h] contiguous.
- * f, p: both NULL, or [rows][h] contiguous buffers that receive act(a) and b act'(a) for the backward call.
+ * f, p: both NULL, or contiguous float [rows][h], 4-byte aligned, that receive act(a) and b act'(a) for the backward call.
  * workspace: 16-byte aligned, marl_gated_workspace_bytes of the same operands (backward 0; NULL where that is 0: 16-byte
  * aligned rows of more than 64, or of weights with many rows, need none). */
 int marl_gated_forward(int32_t dtype, int32_t act, int64_t rows, int32_t d, int32_t h, const void *x, int64_t ldx,
-                       const void *w_gate, int64_t ld_gate, const void *w_up, int64_t ld_up, void *y, void *f, void *p,
+                       const void *w_gate, int64_t ld_gate, const void *w_up, int64_t ld_up, void *y, float *f, float *p,
                        void *workspace, void *stream);
 size_t marl_gated_workspace_bytes(int32_t dtype, int64_t rows, int32_t d, int32_t h, const void *x, int64_t ldx,
                                   const void *w_gate, int64_t ld_gate, const void *w_up, int64_t ld_up, int32_t backward);
@@ -493,7 +493,7 @@ size_t marl_gated_workspace_bytes(int32_t dtype, int64_t rows, int32_t d, int32_
  * forward call.  workspace: 16-byte aligned, marl_gated_workspace_bytes with backward 1 (which is 0 for sizes that the
  * calls refuse). */
 int marl_gated_backward(int32_t dtype, int64_t rows, int32_t d, int32_t h, const void *x, int64_t ldx,
-                        const void *w_gate, int64_t ld_gate, const void *w_up, int64_t ld_up, const void *f, const void *p,
+                        const void *w_gate, int64_t ld_gate, const void *w_up, int64_t ld_up, const float *f, const float *p,
                         const void *gy, int64_t ld_gy, void *dx, void *dw_gate, void *dw_up, void *workspace, void *stream);
 
 /* y = scale x + gate N(block; w_post),  n = N(y; w_pre), with N(v; w) = w (v - mean(v)) / sqrt(var(v) + eps) (MARL_NORM_LAYER)

@@ -14,8 +14,10 @@
 // no transposed copy of a weight or a gradient is ever made.  Chunk positions are permuted within a row (tile_* below) so
 // that the lanes of one LDS access fall on different banks.
 // 16-bit types: v_mfma_f32_32x32x16 with float32 accumulators; float32: v_mfma_f32_32x32x2.  da and db are rounded to
-// the element type, once, because they are matrix operands; f and p are kept in it between forward and backward (T h
-// elements each, against 4 T d h operations for computing a and b again).
+// the element type, once, because they are matrix operands.  f and p are kept between forward and backward in float32, T h
+// elements each, against 4 T d h operations for computing a and b again: in 16 bits da and db would be rounded twice
+// (gradients off by 0.0029 instead of 0.0024 in bf16), and p = b act'(a) may lie outside of float16 where y and the gradients
+// do not.
 // Bound by the matrix cores; FWD / DX / DW measured: T 8192, d 2048, h 8192, bf16: 621 / 465 / 472 us (885 / 1183 / 1165
 // TFLOP/s); T 32768, d 128, h 512, float32: 105 / 80 / 77 us (82 / 108 / 111); T 1999, d 1000, h 2731, float16, operands
 // packed: 50 / 36 / 37 us (436 / 601 / 592).  da and db are bandwidth: 109 us at the first sizes (6.1 TB/s).  Few rows are
@@ -98,29 +100,36 @@ struct ProductArgs {
     int64_t h, half;          // backward: db stands `half` columns behind da (h rounded up to whole chunks)
     int stages;               // stages of k in one slice
     void *out0, *out1;        // FWD: y; DX: dx; DW: dWg, dWu
-    void *save_f, *save_p;    // FWD: NULL, or what backward needs
+    float *save_f, *save_p;   // FWD: NULL, or what backward needs
     float* partial;           // [slices][M][N] when the k range is split
     int act;
     int tiles_m, tiles_n;
 };
 
-// y, and f and p for backward, of `left` (at most a chunk) neighbouring columns from their a and b; stored past the caches,
-// which hold the operands (T 32768, d 128, h 512, float32: 115 -> 103 us)
-template <typename T, int ACT> __device__ __forceinline__ void gate_out(const ProductArgs& args, int64_t at, const float* a, const float* b, int64_t left) {
-    constexpr int CE = Chunk<T>::n;
-    Vec<T> y, vf, vp;
+template <int N> __device__ __forceinline__ void stream_floats(float* p, const float (&v)[N], int64_t left) {
 #pragma unroll
-    for (int e = 0; e < CE; ++e) {
-        float f, df;
-        act_both<ACT, sizeof(T) == 2>(a[e], f, df);
-        y.e[e] = from_f32<T>(f * b[e]);
-        vf.e[e] = from_f32<T>(f);
-        vp.e[e] = from_f32<T>(b[e] * df);
+    for (int c = 0; c < N; c += 4) {
+        const Part<float, 4> t = {{v[c], v[c + 1], v[c + 2], v[c + 3]}};
+        if (left > c) stream_part(p + c, t, left - c);
+    }
+}
+// y, and f and p for backward, of `left` (at most W) neighbouring columns from their a and b; stored past the caches,
+// which hold the operands (T 32768, d 128, h 512, float32: 115 -> 103 us)
+// W columns: a chunk, or four.
+template <typename T, int ACT, int W> __device__ __forceinline__ void gate_out(const ProductArgs& args, int64_t at, const float* a, const float* b, int64_t left) {
+    Part<T, W> y;
+    float f[W], p[W];
+#pragma unroll
+    for (int e = 0; e < W; ++e) {
+        float df;
+        act_both<ACT, sizeof(T) == 2>(a[e], f[e], df);
+        y.e[e] = from_f32<T>(f[e] * b[e]);
+        p[e] = b[e] * df;
     }
     stream_part((T*)args.out0 + at, y, left);
     if (args.save_f) {
-        stream_part((T*)args.save_f + at, vf, left);
-        stream_part((T*)args.save_p + at, vp, left);
+        stream_floats(args.save_f + at, f, left);
+        stream_floats(args.save_p + at, p, left);
     }
 }
 
@@ -446,15 +455,18 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
             for (int v = 0; v < 16; ++v) corner[(8 * (v / 4) + 4 * (lane >> 5) + v % 4) * PITCH + 32 * j + (lane & 31)] = acc[i][j][v];
         const int64_t row0 = m0 + wm * (BM / WM) + 32 * i;
         if constexpr (MODE == FWD) {
-            constexpr int CE = Chunk<T>::n, PER_ROW = COLS / 2 / CE;
+            // f and p are float32: with four columns a lane one store of theirs covers whole lines, with eight (16-bit types)
+            // every other 16 bytes of twice as many.  (The same width without them: the compiler rounds f b to float16 in one
+            // step or in two by what is around it, and y must not depend on whether f and p are kept.)
+            constexpr int W = 4, PER_ROW = COLS / 2 / W;
             by_act(args.act, [&](auto kind) {
                 constexpr int ACT = decltype(kind)::value;
 #pragma unroll 2
                 for (int q = lane; q < 32 * PER_ROW; q += 64) {
-                    const int r = q / PER_ROW, c = q % PER_ROW * CE;                  // c: column among the wave's outputs
+                    const int r = q / PER_ROW, c = q % PER_ROW * W;                   // c: column among the wave's outputs
                     const float* g = corner + r * PITCH + c / 32 * 64 + c % 32;
                     const int64_t m = row0 + r, n = n0 / 2 + wn * (COLS / 2) + c, left = m < args.M ? args.N - n : 0;
-                    if (left > 0) gate_out<T, ACT>(args, m * args.N + n, g, g + 32, left);
+                    if (left > 0) gate_out<T, ACT, W>(args, m * args.N + n, g, g + 32, left);
                 }
             });
         } else if (args.partial) {
@@ -570,7 +582,7 @@ __global__ __launch_bounds__(512) void gated_few_rows_kernel(const ProductArgs a
                     b[e] += part[(((w * MT + t / 32) * 2 + 1) * 16 + v) * 64 + 32 * half + c + e];
                 }
             if (args.partial == nullptr) {
-                gate_out<T, ACT>(args, t * args.N + j0 + c, a, b, args.N - (j0 + c));
+                gate_out<T, ACT, CE>(args, t * args.N + j0 + c, a, b, args.N - (j0 + c));
                 continue;
             }
             float* out = args.partial + (((int64_t)blockIdx.y * args.M + t) * 2) * args.N + j0 + c;
@@ -594,26 +606,30 @@ __global__ __launch_bounds__(256) void gated_finish_kernel(const ProductArgs arg
         for (int e = 0; e < CE; ++e)
             if (j + e < args.N) { a[e] += in[e]; b[e] += in[args.N + e]; }
     }
-    by_act(args.act, [&](auto kind) { gate_out<T, decltype(kind)::value>(args, t * args.N + j, a, b, args.N - j); });
+    by_act(args.act, [&](auto kind) { gate_out<T, decltype(kind)::value, CE>(args, t * args.N + j, a, b, args.N - j); });
 }
 
-// da = gy p and, `half` columns behind it, db = gy f of every row, both padded with zeros: bandwidth (three reads, two writes of T h)
+// da = gy p and, `half` columns behind it, db = gy f of every row, both padded with zeros: bandwidth (reads of f and p in float32
+// and of gy, two writes of T h elements)
 template <typename T, bool WHOLE>
-__global__ __launch_bounds__(256) void gated_da_db_kernel(const T* __restrict__ f, const T* __restrict__ p, const T* __restrict__ gy, int64_t ldgy,
+__global__ __launch_bounds__(256) void gated_da_db_kernel(const float* __restrict__ f, const float* __restrict__ p, const T* __restrict__ gy, int64_t ldgy,
                                                            T* __restrict__ dab, int64_t half, int64_t rows, int64_t h) {
     constexpr int CE = Chunk<T>::n;
     const int64_t per = (h + CE - 1) / CE;
     for (int64_t t = blockIdx.y; t < rows; t += gridDim.y)
         for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < per; q += (int64_t)gridDim.x * 256) {
             const int64_t c = q * CE;
-            auto load = [&](const T* row) { return WHOLE ? load_chunk(row + c) : load_clipped(row, c, h); };
-            const Vec<T> vf = load(f + t * h), vp = load(p + t * h), vg = load(gy + t * ldgy);
+            auto load = [&](auto* row, int64_t at) { return WHOLE ? load_chunk(row + at) : load_clipped(row, at, h); };
+            Vec<float> vf[CE / 4], vp[CE / 4];
+#pragma unroll
+            for (int k = 0; k < CE / 4; ++k) { vf[k] = load(f + t * h, c + 4 * k); vp[k] = load(p + t * h, c + 4 * k); }
+            const Vec<T> vg = load(gy + t * ldgy, c);
             Vec<T> da, db;
 #pragma unroll
             for (int i = 0; i < CE; ++i) {
                 const float g = to_f32(vg.e[i]);
-                da.e[i] = from_f32<T>(g * to_f32(vp.e[i]));
-                db.e[i] = from_f32<T>(g * to_f32(vf.e[i]));
+                da.e[i] = from_f32<T>(g * vp[i / 4].e[i % 4]);
+                db.e[i] = from_f32<T>(g * vf[i / 4].e[i % 4]);
             }
             *(Vec<T>*)(dab + t * 2 * half + c) = da;                // zeros behind h
             *(Vec<T>*)(dab + t * 2 * half + half + c) = db;
@@ -739,7 +755,7 @@ template <typename T> size_t workspace(const Gated& g, bool backward) {
     return packed + (size_t)(round_256(g.rows * h2 * (int64_t)sizeof(T)) + (sx > sw ? sx : sw) * (int64_t)sizeof(float));
 }
 
-template <typename T> int forward(int act, Gated g, void* y, void* f, void* p, void* workspace, hipStream_t stream) {
+template <typename T> int forward(int act, Gated g, void* y, float* f, float* p, void* workspace, hipStream_t stream) {
     ProductArgs a = {};
     char* ws = (char*)workspace;
     if (g.rows > FEW_ROWS) { g.x = pack<T>(g.x, g.d, ws, stream); g.wg = pack<T>(g.wg, g.d, ws, stream); g.wu = pack<T>(g.wu, g.d, ws, stream); }
@@ -754,7 +770,7 @@ template <typename T> int forward(int act, Gated g, void* y, void* f, void* p, v
     return MARL_EHIP;
 }
 
-template <typename T> int backward(Gated g, const void* f, const void* p, const void* gy, int64_t ldgy, void* dx, void* dwg, void* dwu,
+template <typename T> int backward(Gated g, const float* f, const float* p, const void* gy, int64_t ldgy, void* dx, void* dwg, void* dwu,
                                    void* workspace, hipStream_t stream) {
     char* ws = (char*)workspace;
     const int64_t half = packed_ld<T>(g.h), per = half / Chunk<T>::n;
@@ -762,7 +778,7 @@ template <typename T> int backward(Gated g, const void* f, const void* p, const 
     ws += round_256(g.rows * 2 * half * (int64_t)sizeof(T));
     auto* da_db = g.h % Chunk<T>::n == 0 ? gated_da_db_kernel<T, true> : gated_da_db_kernel<T, false>;
     hipLaunchKernelGGL(da_db, dim3((unsigned)((per + 255) / 256), (unsigned)(g.rows < 65535 ? g.rows : 65535)), dim3(256), 0, stream,
-                       (const T*)f, (const T*)p, (const T*)gy, ldgy, dab, half, g.rows, (int64_t)g.h);
+                       f, p, (const T*)gy, ldgy, dab, half, g.rows, (int64_t)g.h);
     hipError_t err = hipGetLastError();
     if (err == hipSuccess && dx) {                // DX moves through both weights with one stride
         const bool both = g.wg.ld != g.wu.ld || !aligned<T>(g.wg, g.d) || !aligned<T>(g.wu, g.d);
@@ -804,7 +820,7 @@ int check_sizes(int32_t dtype, int32_t act, int64_t rows, int32_t d, int32_t h) 
 extern "C" {
 
 int marl_gated_forward(int32_t dtype, int32_t act, int64_t rows, int32_t d, int32_t h, const void* x, int64_t ldx, const void* w_gate,
-                       int64_t ld_gate, const void* w_up, int64_t ld_up, void* y, void* f, void* p, void* workspace_, void* stream) {
+                       int64_t ld_gate, const void* w_up, int64_t ld_up, void* y, float* f, float* p, void* workspace_, void* stream) {
     const int rc = check_sizes(dtype, act, rows, d, h);
     if (rc != MARL_OK) return rc;
     if (!x || !w_gate || !w_up || !y || (f == nullptr) != (p == nullptr) || ((uintptr_t)workspace_ & 15)) return MARL_EINVAL;
@@ -823,7 +839,7 @@ size_t marl_gated_workspace_bytes(int32_t dtype, int64_t rows, int32_t d, int32_
 }
 
 int marl_gated_backward(int32_t dtype, int64_t rows, int32_t d, int32_t h, const void* x, int64_t ldx, const void* w_gate,
-                        int64_t ld_gate, const void* w_up, int64_t ld_up, const void* f, const void* p, const void* gy, int64_t ld_gy,
+                        int64_t ld_gate, const void* w_up, int64_t ld_up, const float* f, const float* p, const void* gy, int64_t ld_gy,
                         void* dx, void* dw_gate, void* dw_up, void* workspace_, void* stream) {
     const int rc = check_sizes(dtype, MARL_ACT_SILU, rows, d, h);
     if (rc != MARL_OK) return rc;

@@ -138,7 +138,7 @@ Tensor3 gated_launch(const Tensor& x, const Tensor& wg, const Tensor& wu, c10::s
     const auto shape = check_gated(x, wg, wu, act);
     same_device("gated_linear", x, {&wg, &wu});
     Tensor y = at::empty(shape, x.options()), f, p;
-    if (save) { f = at::empty(shape, x.options()); p = at::empty(shape, x.options()); }
+    if (save) { f = at::empty(shape, x.options().dtype(at::kFloat)); p = at::empty_like(f); }
     if (y.numel()) {
         const Rows rx(x), rg(wg), ru(wu);
         const On on(x);
@@ -147,7 +147,7 @@ Tensor3 gated_launch(const Tensor& x, const Tensor& wg, const Tensor& wu, c10::s
         const size_t bytes = lib.marl_gated_workspace_bytes(dt, rx.n, d, h, rx.p(), rx.ld, rg.p(), rg.ld, ru.p(), ru.ld, 0);
         Tensor ws = bytes ? scratch(x, bytes) : Tensor();
         check(lib.marl_gated_forward(dt, act_code(act), rx.n, d, h, rx.p(), rx.ld, rg.p(), rg.ld, ru.p(), ru.ld, y.mutable_data_ptr(),
-                                     save ? f.mutable_data_ptr() : nullptr, save ? p.mutable_data_ptr() : nullptr,
+                                     save ? f.mutable_data_ptr<float>() : nullptr, save ? p.mutable_data_ptr<float>() : nullptr,
                                      bytes ? ws.mutable_data_ptr() : nullptr, on.stream), "marl_gated_forward");
     }
     return {y, f, p};
@@ -160,7 +160,8 @@ void check_gated_backward(const Tensor& gy, const Tensor& x, const Tensor& wg, c
     TORCH_CHECK_VALUE(gy.sizes() == at::IntArrayRef(shape), "gated_linear: gy must be shaped like the result");
     check_kept("gated_linear", f, shape);
     check_kept("gated_linear", p, shape);
-    same_type("gated_linear", x, {&gy, &f, &p});
+    TORCH_CHECK_VALUE(f.scalar_type() == at::kFloat && p.scalar_type() == at::kFloat, "gated_linear: f and p must be float32");
+    same_type("gated_linear", x, {&gy});
 }
 
 Tensor3 gated_linear_backward(const Tensor& gy, const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& f, const Tensor& p, bool need_x, bool need_w) {
@@ -174,8 +175,8 @@ Tensor3 gated_linear_backward(const Tensor& gy, const Tensor& x, const Tensor& w
     const On on(x);
     const int dt = type_code(x);
     Tensor ws = scratch(x, lib.marl_gated_workspace_bytes(dt, rx.n, (int32_t)d, (int32_t)h, rx.p(), rx.ld, rg.p(), rg.ld, ru.p(), ru.ld, 1));
-    check(lib.marl_gated_backward(dt, rx.n, (int32_t)d, (int32_t)h, rx.p(), rx.ld, rg.p(), rg.ld, ru.p(), ru.ld, f.const_data_ptr(),
-                                  p.const_data_ptr(), rgy.p(), rgy.ld, need_x ? dx.mutable_data_ptr() : nullptr,
+    check(lib.marl_gated_backward(dt, rx.n, (int32_t)d, (int32_t)h, rx.p(), rx.ld, rg.p(), rg.ld, ru.p(), ru.ld, f.const_data_ptr<float>(),
+                                  p.const_data_ptr<float>(), rgy.p(), rgy.ld, need_x ? dx.mutable_data_ptr() : nullptr,
                                   need_w ? dg.mutable_data_ptr() : nullptr, need_w ? du.mutable_data_ptr() : nullptr, ws.mutable_data_ptr(),
                                   on.stream), "marl_gated_backward");
     return {dx, dg, du};
@@ -183,7 +184,8 @@ Tensor3 gated_linear_backward(const Tensor& gy, const Tensor& x, const Tensor& w
 
 Tensor gated_linear_meta(const Tensor& x, const Tensor& wg, const Tensor& wu, c10::string_view act) { return at::empty(check_gated(x, wg, wu, act), x.options()); }
 Tensor3 gated_linear_saved_meta(const Tensor& x, const Tensor& wg, const Tensor& wu, c10::string_view act) {
-    return {gated_linear_meta(x, wg, wu, act), gated_linear_meta(x, wg, wu, act), gated_linear_meta(x, wg, wu, act)};
+    const Tensor y = gated_linear_meta(x, wg, wu, act);
+    return {y, at::empty_like(y, at::kFloat), at::empty_like(y, at::kFloat)};
 }
 Tensor3 gated_linear_backward_meta(const Tensor& gy, const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& f, const Tensor& p, bool need_x, bool need_w) {
     check_gated_backward(gy, x, wg, wu, f, p);

@@ -64,12 +64,19 @@ template <typename T> __device__ __forceinline__ Vec<T> load_clipped(const T* ro
     for (int e = 0; e < CE; ++e) v.e[e] = e + by < CE ? v.e[e] : (T)0.0f;
     return v;
 }
-// store_part for results that nothing reads soon: past the caches
-template <typename T> __device__ __forceinline__ void stream_part(T* p, const Vec<T>& v, int64_t left) {
-    constexpr int n = Chunk<T>::n;
-    if (left >= n) { __builtin_nontemporal_store(__builtin_bit_cast(uint4v, v), &((Unaligned*)p)->v); return; }
+// N elements, 8 or 16 bytes.  stream_part: store_part for results that nothing reads soon, past the caches
+template <typename T, int N> struct alignas(N * sizeof(T)) Part { T e[N]; };
+typedef unsigned int uint2v __attribute__((ext_vector_type(2)));
+struct __attribute__((packed, aligned(2))) Unaligned8 { uint2v v; };
+template <typename T, int N> __device__ __forceinline__ void stream_part(T* p, const Part<T, N>& v, int64_t left) {
+    static_assert(N * sizeof(T) == 16 || N * sizeof(T) == 8, "one store");
+    if (left >= N) {
+        if constexpr (N * sizeof(T) == 16) __builtin_nontemporal_store(__builtin_bit_cast(uint4v, v), &((Unaligned*)p)->v);
+        else __builtin_nontemporal_store(__builtin_bit_cast(uint2v, v), &((Unaligned8*)p)->v);
+        return;
+    }
 #pragma unroll
-    for (int i = 0; i < n; ++i) if (i < left) p[i] = v.e[i];
+    for (int i = 0; i < N; ++i) if (i < left) p[i] = v.e[i];
 }
 
 }  // namespace marl_types
