@@ -1027,7 +1027,10 @@ class PPOAgent:
     def export_actor(self, path):
         """`actor_state_dict.pt` for the reference's deployment controller (deploy.py:139-188): the state
         dict its MinimalActor (deploy.py:33-92) loads strictly, i.e. trunk, velocity-mean head and band
-        head; the log-std head is not part of the deployed network."""
+        head; the log-std head is not part of the deployed network.  An actor with another trunk is refused:
+        MinimalActor has the mlp one only."""
+        if self.trunk != "mlp":
+            raise ValueError(f'export_actor: the deployment actor has trunk="mlp", not {self.trunk!r}')
         path = Path(path)
         path.parent.mkdir(parents=True, exist_ok=True)
         sd = {k: v.detach().cpu().clone() for k, v in self.actor.state_dict().items()

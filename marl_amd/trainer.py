@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import csv
 import json
+import logging
 import time
 from collections import deque
 from pathlib import Path
@@ -24,6 +25,8 @@ import torch
 from . import _lib
 from .agents import PPOAgent, _dist_on
 from .env import BatchedJammerEnv, EnvConfig
+
+_log = logging.getLogger(__name__)
 
 # column names of training_log.csv / history.json (training/metrics.py:121-135)
 HISTORY_KEYS = ("timestep", "episode", "reward", "lambda2_reduction", "episode_length", "band_match_rate",
@@ -263,14 +266,17 @@ class BatchedTrainer:
     # -- checkpoints (training/trainer.py:387-420) ----------------------------------
     def save_checkpoint(self, name: str = "checkpoint", directory: Optional[str] = None) -> Path:
         """ppo_agent.pt + trainer_state.json as the reference writes them, the deployment actor
-        (actor_state_dict.pt, deploy.py:139-188), and env_state_<rank>.pt: the device state of the E
+        (actor_state_dict.pt, deploy.py:139-188; trunk="mlp" only), and env_state_<rank>.pt: the device state of the E
         environments, the current observation and the generator counters, so that a resumed run continues
         the same trajectory.  Every rank writes its own env state; rank 0 writes the rest."""
         base = Path(directory) if directory is not None else (self.output_dir or Path(".")) / "checkpoints" / name
         base.mkdir(parents=True, exist_ok=True)
         if self.rank == 0:
             self.agent.save(base)
-            self.agent.export_actor(base / "actor_state_dict.pt")
+            if self.agent.trunk == "mlp":
+                self.agent.export_actor(base / "actor_state_dict.pt")
+            else:
+                _log.warning("actor_state_dict.pt not written: the deployment actor has trunk='mlp', not %r", self.agent.trunk)
             with open(base / "trainer_state.json", "w") as f:
                 json.dump({"total_timesteps": self.total_timesteps, "total_episodes": self.total_episodes,
                            "total_rollouts": self.total_rollouts, "best_reduction": self.best_reduction,

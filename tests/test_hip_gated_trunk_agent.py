@@ -1,0 +1,30 @@
+"""GPU tests of an agent with a gated trunk around its training loop: what is exported, the dropout seed, rows outside of the
+rollout buffer."""
+import logging
+
+import pytest
+import torch
+
+from marl_amd import EnvConfig
+from marl_amd.agents import PPOAgent
+from marl_amd.trainer import BatchedTrainer
+
+pytestmark = pytest.mark.gpu
+
+
+def agent_of(**kw):
+    return PPOAgent(**{**dict(device="cuda", M=2, num_envs=3, rollout_length=2, trunk="gated", trunk_blocks=1, trunk_dropout=0.3, hidden_dim=32), **kw})
+
+
+def test_a_gated_actor_is_not_exported_for_deployment(tmp_path, caplog):
+    with pytest.raises(ValueError, match="mlp"):
+        agent_of().export_actor(tmp_path / "a" / "actor_state_dict.pt")
+    assert not (tmp_path / "a").exists()
+    cfg = EnvConfig.fast_preset(N=10, M=2)
+    for trunk, written in (("gated", False), ("mlp", True)):
+        tr = BatchedTrainer(cfg, 4, rollout_length=2, seed=1, agent_kwargs=dict(trunk=trunk, hidden_dim=64, n_epochs=1), log_step_info=False)
+        caplog.clear()
+        with caplog.at_level(logging.WARNING):
+            base = tr.save_checkpoint(directory=str(tmp_path / trunk))
+        assert (base / "ppo_agent.pt").exists() and (base / "actor_state_dict.pt").exists() == written
+        assert any("actor_state_dict" in r.getMessage() for r in caplog.records) != written
