@@ -102,6 +102,12 @@ class GatedBlock(nn.Module):
         return ops.residual_norm(x, self.down(h), self.post, self.pre, self.gate, 1.0, 1e-5, "layer")
 
 
+def _dropout_seed(seed: int) -> int:
+    """Seed of a trunk's first block (block i adds i) for a program's seed: the operator takes int64, torch.manual_seed any
+    64 bits."""
+    return (int(seed) << 8) % (1 << 63)
+
+
 class GatedTrunk(nn.Module):
     """obs -> hidden -> `blocks` residual blocks (GatedBlock), the features normalised.  Runs on the GPU only.
 
@@ -530,7 +536,7 @@ class PPOAgent:
         if not 0.0 <= self.trunk_dropout < 1.0 or (self.trunk_dropout > 0.0 and trunk != "gated"):
             raise ValueError('trunk_dropout must be in [0, 1), and needs trunk="gated"')
         self.actor = Actor(obs_dim, hidden_dim, v_max, num_bands, log_std_min, log_std_max, trunk, trunk_blocks, trunk_dropout,
-                           dropout_seed=0 if seed is None else int(seed) << 8).to(self.device)
+                           dropout_seed=0 if seed is None else _dropout_seed(seed)).to(self.device)
         self.critic = Critic(obs_dim, hidden_dim, trunk, trunk_blocks).to(self.device)
         if _dist_on():                       # every rank starts from rank 0's weights
             for p in list(self.actor.parameters()) + list(self.critic.parameters()):

@@ -28,3 +28,10 @@ def test_a_gated_actor_is_not_exported_for_deployment(tmp_path, caplog):
             base = tr.save_checkpoint(directory=str(tmp_path / trunk))
         assert (base / "ppo_agent.pt").exists() and (base / "actor_state_dict.pt").exists() == written
         assert any("actor_state_dict" in r.getMessage() for r in caplog.records) != written
+
+
+@pytest.mark.parametrize("seed", [(1 << 55) + 3, (1 << 63) - 1, -1, 7])
+def test_every_seed_that_torch_takes_gives_a_dropout_seed(seed):
+    a = agent_of(seed=seed)
+    actions, logp, _ = a.get_action(torch.rand(3, 2, 5, device="cuda"))
+    assert bool(logp.isfinite().all()) and 0 <= a.actor.trunk.dropout_seed < 1 << 63
