@@ -102,10 +102,11 @@ class GatedBlock(nn.Module):
         return ops.residual_norm(x, self.down(h), self.post, self.pre, self.gate, 1.0, 1e-5, "layer")
 
 
-def _dropout_seed(seed: int) -> int:
+def _dropout_seed(seed: Optional[int]) -> int:
     """Seed of a trunk's first block (block i adds i) for a program's seed: the operator takes int64, torch.manual_seed any
-    64 bits."""
-    return (int(seed) << 8) % (1 << 63)
+    64 bits.  None: drawn from torch's default generator, as the weights are."""
+    seed = int(torch.randint(1 << 55, ())) if seed is None else int(seed)
+    return (seed << 8) % (1 << 63)
 
 
 class GatedTrunk(nn.Module):
@@ -536,7 +537,7 @@ class PPOAgent:
         if not 0.0 <= self.trunk_dropout < 1.0 or (self.trunk_dropout > 0.0 and trunk != "gated"):
             raise ValueError('trunk_dropout must be in [0, 1), and needs trunk="gated"')
         self.actor = Actor(obs_dim, hidden_dim, v_max, num_bands, log_std_min, log_std_max, trunk, trunk_blocks, trunk_dropout,
-                           dropout_seed=0 if seed is None else _dropout_seed(seed)).to(self.device)
+                           dropout_seed=_dropout_seed(seed) if trunk == "gated" else 0).to(self.device)
         self.critic = Critic(obs_dim, hidden_dim, trunk, trunk_blocks).to(self.device)
         if _dist_on():                       # every rank starts from rank 0's weights
             for p in list(self.actor.parameters()) + list(self.critic.parameters()):

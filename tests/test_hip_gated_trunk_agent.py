@@ -35,3 +35,12 @@ def test_every_seed_that_torch_takes_gives_a_dropout_seed(seed):
     a = agent_of(seed=seed)
     actions, logp, _ = a.get_action(torch.rand(3, 2, 5, device="cuda"))
     assert bool(logp.isfinite().all()) and 0 <= a.actor.trunk.dropout_seed < 1 << 63
+
+
+def test_agents_without_a_seed_have_masks_of_their_own():
+    torch.manual_seed(11)
+    a = agent_of().actor.trunk.dropout_seed
+    torch.manual_seed(12)
+    b = agent_of().actor.trunk.dropout_seed
+    torch.manual_seed(11)
+    assert a != b and agent_of().actor.trunk.dropout_seed == a
