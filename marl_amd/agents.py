@@ -964,11 +964,14 @@ class PPOAgent:
         path = Path(path)
         path.mkdir(parents=True, exist_ok=True)
         stats = {k: [float(x) for x in v] for k, v in self.training_stats.items()}
-        torch.save({"actor_state_dict": self.actor.state_dict(), "critic_state_dict": self.critic.state_dict(),
-                    "actor_optimizer_state_dict": self._portable_optimizer_state(self.actor_optimizer),
-                    "critic_optimizer_state_dict": self._portable_optimizer_state(self.critic_optimizer),
-                    "total_timesteps": self.total_timesteps, "total_updates": self.total_updates,
-                    "training_stats": stats, "config": self._config()}, path / "ppo_agent.pt")
+        ck = {"actor_state_dict": self.actor.state_dict(), "critic_state_dict": self.critic.state_dict(),
+              "actor_optimizer_state_dict": self._portable_optimizer_state(self.actor_optimizer),
+              "critic_optimizer_state_dict": self._portable_optimizer_state(self.critic_optimizer),
+              "total_timesteps": self.total_timesteps, "total_updates": self.total_updates,
+              "training_stats": stats, "config": self._config()}
+        if self.actor.gated:                     # a resumed run goes on with the masks of this one
+            ck["trunk_dropout_seed"] = self.actor.trunk.dropout_seed
+        torch.save(ck, path / "ppo_agent.pt")
 
     @staticmethod
     def _portable_optimizer_state(opt):
@@ -1028,6 +1031,8 @@ class PPOAgent:
         if self._fz is not None:                       # the loaded moments into the flat vectors marl_ppo_apply steps
             self._flatten_optimizer_state()
         self._packed_stale = True
+        if self.actor.gated and "trunk_dropout_seed" in ck:
+            self.actor.trunk.dropout_seed = int(ck["trunk_dropout_seed"])
         if self._row_base is not None:
             self._set_row_base()
 

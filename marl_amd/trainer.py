@@ -133,6 +133,7 @@ class BatchedTrainer:
         self._done = torch.zeros(num_envs, dtype=torch.bool, device=self.device)
         self.use_graph = bool(use_graph) and self.device.type == "cuda"
         self._graph = None
+        self._graph_seed = None           # dropout seed that the captured launches hold
         self._eager_rollouts = 0
         # episodes, sum of returns, sum of lambda2 reductions (%), sum of lengths: filled by the step kernels
         self._stats = torch.zeros(4, dtype=torch.float64, device=self.device)
@@ -175,6 +176,9 @@ class BatchedTrainer:
             self._rollout_steps()                          # first rollout eagerly: warms up every lazy initialisation
             self._eager_rollouts += 1
         else:
+            seed = agent.actor.trunk.dropout_seed if agent.actor.gated else None
+            if self._graph is not None and seed != self._graph_seed:
+                self._graph = None                         # an agent was loaded: captured again
             if self._graph is None:
                 pos, steps, calls = agent.buffer.pos, agent.total_timesteps, agent._act_calls
                 if agent.policy_kernel:
@@ -183,7 +187,7 @@ class BatchedTrainer:
                 g = torch.cuda.CUDAGraph()
                 with torch.cuda.graph(g):
                     self._rollout_steps()
-                self._graph = g
+                self._graph, self._graph_seed = g, seed
                 # capture runs nothing: put the host-side counters back and replay below
                 agent.buffer.pos, agent.buffer.full, agent.total_timesteps = pos, False, steps
                 agent._act_calls = calls
@@ -298,7 +302,8 @@ class BatchedTrainer:
 
     def load_checkpoint(self, path: str):
         """Restores what save_checkpoint wrote (the agent in place, counters, environments).  The captured
-        rollout graph of this object, if any, stays valid: every buffer is restored in place."""
+        rollout graph of this object, if any, stays valid: every buffer is restored in place.  (Not with another
+        dropout seed, which its launches hold: the next rollout is captured again.)"""
         base = Path(path)
         self.agent.load(base)
         if self.agent.buffer is not None:

@@ -44,3 +44,37 @@ def test_agents_without_a_seed_have_masks_of_their_own():
     b = agent_of().actor.trunk.dropout_seed
     torch.manual_seed(11)
     assert a != b and agent_of().actor.trunk.dropout_seed == a
+
+
+def test_a_checkpoint_keeps_the_dropout_seed(tmp_path):
+    a = agent_of(seed=5)
+    a.save(tmp_path)
+    b, c = PPOAgent.from_checkpoint(tmp_path, device="cuda", num_envs=3), agent_of(seed=6)
+    c.load(tmp_path)
+    obs, keys = torch.rand(3, 2, 5, device="cuda"), torch.arange(6, device="cuda").view(3, 2)
+    want = a.actor(obs, keys)
+    for other in (b, c):
+        assert all(torch.equal(p, q) for p, q in zip(want, other.actor(obs, keys)))
+
+
+def test_a_captured_rollout_goes_on_with_the_loaded_dropout_seed(tmp_path):
+    cfg = EnvConfig.fast_preset(N=10, M=2)
+    make = lambda seed: BatchedTrainer(cfg, 8, rollout_length=4, seed=seed, minibatches_per_epoch=2, log_step_info=False,
+                                       agent_kwargs=dict(trunk="gated", trunk_dropout=0.3, hidden_dim=64, n_epochs=1))
+    first, second = make(2), make(3)
+    first.collect_rollout()
+    first.update()
+    first.save_checkpoint(directory=str(tmp_path))
+    for _ in range(3):                           # eager, captured, replayed
+        second.collect_rollout()
+        second.update()
+    second.load_checkpoint(str(tmp_path))
+    for _ in range(2):
+        second.collect_rollout()
+        agent = second.agent
+        obs, actions, old, *_ = agent.buffer.get_samples()
+        with torch.no_grad():
+            lp, _ = agent.actor.evaluate_actions(obs, actions, torch.arange(obs.shape[0], device="cuda") + agent._row_base)
+        inside = actions[:, :2].abs().max(1).values < cfg.v_max
+        assert int(inside.sum()) > 10 and float((lp - old)[inside].abs().max()) < 1e-4       # the same float32 networks
+        second.update()
