@@ -587,9 +587,13 @@ class PPOAgent:
         self._row_base.fill_((rank << 48) + self.total_updates * self.rollout_length * self.E * self.M)
 
     def _slot_keys(self, obs):
-        """Dropout keys of the rows acted on now, those of the buffer's current slot; None where no dropout applies."""
-        if self._row_base is None or not self.actor.training or tuple(obs.shape[:2]) != (self.E, self.M):
+        """Dropout keys of the rows acted on now, those of the buffer's current slot; None where no dropout applies.  Other
+        rows than the buffer's have no keys: drawn without dropout, they would meet masks in an update."""
+        if self._row_base is None or not self.actor.training:
             return None
+        if tuple(obs.shape[:2]) != (self.E, self.M):
+            raise ValueError(f"acting with trunk_dropout in training mode takes observations of {(self.E, self.M)} rows, not "
+                             f"{tuple(obs.shape[:2])}; set_training_mode(False) acts on any rows, without dropout")
         return self._row_number + (self._row_base + self.buffer.pos * self.E * self.M)
 
     @torch.no_grad()

@@ -78,3 +78,13 @@ def test_a_captured_rollout_goes_on_with_the_loaded_dropout_seed(tmp_path):
         inside = actions[:, :2].abs().max(1).values < cfg.v_max
         assert int(inside.sum()) > 10 and float((lp - old)[inside].abs().max()) < 1e-4       # the same float32 networks
         second.update()
+
+
+def test_rows_outside_of_the_buffer_are_refused_while_dropout_is_on():
+    a = agent_of(seed=1)
+    for shape in ((4, 2, 5), (3, 1, 5), (2, 5)):
+        with pytest.raises(ValueError, match="set_training_mode"):
+            a.get_action(torch.rand(*shape, device="cuda"))
+    a.set_training_mode(False)
+    assert a.get_action(torch.rand(4, 2, 5, device="cuda"))[0].shape == (4, 2, 3)
+    assert agent_of(seed=1, trunk_dropout=0.0).get_action(torch.rand(4, 2, 5, device="cuda"))[0].shape == (4, 2, 3)
