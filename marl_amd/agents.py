@@ -211,6 +211,8 @@ class Critic(nn.Module):
     def __init__(self, obs_dim=5, hidden_dim=128, trunk="mlp", trunk_blocks=2):
         super().__init__()
         self.obs_dim, self.hidden_dim = obs_dim, hidden_dim
+        if trunk not in ("mlp", "gated"):
+            raise ValueError(f"trunk must be mlp or gated, not {trunk!r}")
         if trunk == "gated":
             self.network = nn.Sequential(GatedTrunk(obs_dim, hidden_dim, trunk_blocks), TallLinear(hidden_dim, 1))
         else:
