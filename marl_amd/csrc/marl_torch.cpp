@@ -111,9 +111,10 @@ template <class F> const auto& handle(const char* name) {
     return h;
 }
 
+// true also for forward-mode tangents, which the autograd functions refuse; below them they would be dropped
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
-    if (!c10::GradMode::is_enabled()) return false;
-    for (const Tensor* t : ts) if (t && t->defined() && t->requires_grad()) return true;
+    for (const Tensor* t : ts)
+        if (t && t->defined() && ((c10::GradMode::is_enabled() && t->requires_grad()) || t->_fw_grad(0).defined())) return true;
     return false;
 }
 
