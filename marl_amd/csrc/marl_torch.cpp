@@ -106,10 +106,12 @@ variable_list once(variable_list g, const char* op) {
     return (*error)(std::move(g));
 }
 
-template <class F> const auto& handle(const char* name) {
-    static const auto h = c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
-    return h;
-}
+// the operator of this name and signature, looked up once for every place that names it
+#define MARL_OP(name, ...)                                                                                                   \
+    ([]() -> const c10::TypedOperatorHandle<__VA_ARGS__>& {                                                                  \
+        static const auto h = c10::Dispatcher::singleton().findSchemaOrThrow("marl_amd::" name, "").typed<__VA_ARGS__>();     \
+        return h;                                                                                                            \
+    }())
 
 // true also for forward-mode tangents, which the autograd functions refuse; below them they would be dropped
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
@@ -197,22 +199,21 @@ Tensor3 gated_linear_backward_meta(const Tensor& gy, const Tensor& x, const Tens
 struct GatedLinear : torch::autograd::Function<GatedLinear> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& wg, const Tensor& wu, std::string act) {
         at::AutoDispatchBelowADInplaceOrView below;
-        auto [y, f, p] = handle<Tensor3(const Tensor&, const Tensor&, const Tensor&, c10::string_view)>("marl_amd::gated_linear_saved").call(x, wg, wu, act);
+        auto [y, f, p] = MARL_OP("gated_linear_saved", Tensor3(const Tensor&, const Tensor&, const Tensor&, c10::string_view)).call(x, wg, wu, act);
         ctx->save_for_backward({x, wg, wu, f, p});
         return y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list g) {
         const auto s = ctx->get_saved_variables();
         const bool nx = ctx->needs_input_grad(0), ng = ctx->needs_input_grad(1), nu = ctx->needs_input_grad(2);
-        auto [dx, dg, du] = handle<Tensor3(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, bool, bool)>(
-            "marl_amd::gated_linear_backward").call(g[0], s[0], s[1], s[2], s[3], s[4], nx, ng || nu);
+        auto [dx, dg, du] = MARL_OP("gated_linear_backward", Tensor3(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, bool, bool)).call(g[0], s[0], s[1], s[2], s[3], s[4], nx, ng || nu);
         return once({nx ? dx : Tensor(), ng ? dg : Tensor(), nu ? du : Tensor(), Tensor()}, "gated_linear");
     }
 };
 Tensor gated_linear_autograd(const Tensor& x, const Tensor& wg, const Tensor& wu, c10::string_view act) {
     if (wants_grad({&x, &wg, &wu})) return GatedLinear::apply(x, wg, wu, std::string(act));
     at::AutoDispatchBelowADInplaceOrView below;
-    return handle<Tensor(const Tensor&, const Tensor&, const Tensor&, c10::string_view)>("marl_amd::gated_linear").call(x, wg, wu, act);
+    return MARL_OP("gated_linear", Tensor(const Tensor&, const Tensor&, const Tensor&, c10::string_view)).call(x, wg, wu, act);
 }
 
 // -- residual_norm -----------------------------------------------------------------------------------------------------
@@ -324,8 +325,7 @@ Tensor5 residual_norm_backward_meta(const optional<Tensor>& gy, const optional<T
 struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& block, const Tensor& wpost, const Tensor& wpre, const optional<Tensor>& gate, double scale, double eps, std::string kind) {
         at::AutoDispatchBelowADInplaceOrView below;
-        auto [y, n, stats] = handle<Tensor3(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const optional<Tensor>&, double, double, c10::string_view)>(
-            "marl_amd::residual_norm_saved").call(x, block, wpost, wpre, gate, scale, eps, kind);
+        auto [y, n, stats] = MARL_OP("residual_norm_saved", Tensor3(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const optional<Tensor>&, double, double, c10::string_view)).call(x, block, wpost, wpre, gate, scale, eps, kind);
         ctx->save_for_backward({x, block, wpost, wpre, gate ? *gate : Tensor(), stats});
         ctx->saved_data["scale"] = scale;
         ctx->saved_data["kind"] = kind;
@@ -336,9 +336,7 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         if (!g[0].defined() && !g[1].defined()) return variable_list(8);
         const auto s = ctx->get_saved_variables();
         const auto given = [](const Tensor& t) { return t.defined() ? optional<Tensor>(t) : optional<Tensor>(); };
-        auto [dx, db, dpost, dpre, dgate] = handle<Tensor5(const optional<Tensor>&, const optional<Tensor>&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
-                                                           const optional<Tensor>&, const Tensor&, double, c10::string_view)>("marl_amd::residual_norm_backward")
-            .call(given(g[0]), given(g[1]), s[0].contiguous(), s[1], s[2], s[3], given(s[4]), s[5], ctx->saved_data["scale"].toDouble(), ctx->saved_data["kind"].toStringRef());
+        auto [dx, db, dpost, dpre, dgate] = MARL_OP("residual_norm_backward", Tensor5(const optional<Tensor>&, const optional<Tensor>&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const optional<Tensor>&, const Tensor&, double, c10::string_view)).call(given(g[0]), given(g[1]), s[0].contiguous(), s[1], s[2], s[3], given(s[4]), s[5], ctx->saved_data["scale"].toDouble(), ctx->saved_data["kind"].toStringRef());
         variable_list out = {dx, db, dpost, dpre, s[4].defined() ? dgate : Tensor(), Tensor(), Tensor(), Tensor()};
         for (size_t i = 0; i < (s[4].defined() ? 5 : 4); ++i) if (!ctx->needs_input_grad(i)) out[i] = Tensor();
         return once(std::move(out), "residual_norm");
@@ -350,8 +348,7 @@ Tensor2 residual_norm_autograd(const Tensor& x, const Tensor& block, const Tenso
         return {o[0], o[1]};
     }
     at::AutoDispatchBelowADInplaceOrView below;
-    return handle<Tensor2(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const optional<Tensor>&, double, double, c10::string_view)>("marl_amd::residual_norm")
-        .call(x, block, wpost, wpre, gate, scale, eps, kind);
+    return MARL_OP("residual_norm", Tensor2(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const optional<Tensor>&, double, double, c10::string_view)).call(x, block, wpost, wpre, gate, scale, eps, kind);
 }
 
 // -- keyed_dropout -----------------------------------------------------------------------------------------------------
@@ -380,7 +377,7 @@ Tensor keyed_dropout_meta(const Tensor& x, double p, int64_t, const optional<Ten
     return at::empty(x.sizes(), x.options());
 }
 Tensor call_dropout(const Tensor& x, double p, int64_t seed, const optional<Tensor>& keys) {
-    return handle<Tensor(const Tensor&, double, int64_t, const optional<Tensor>&)>("marl_amd::keyed_dropout").call(x, p, seed, keys);
+    return MARL_OP("keyed_dropout", Tensor(const Tensor&, double, int64_t, const optional<Tensor>&)).call(x, p, seed, keys);
 }
 struct KeyedDropout : torch::autograd::Function<KeyedDropout> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, double p, int64_t seed, const optional<Tensor>& keys) {
@@ -439,8 +436,7 @@ Tensor2 sample_logits_meta(const Tensor& logits, const Tensor& u, double tempera
 // not differentiable: its outputs are constants to autograd
 Tensor2 sample_logits_autograd(const Tensor& logits, const Tensor& u, double temperature, int64_t top_k, double top_p, double min_p, const optional<Tensor>& settings) {
     at::AutoDispatchBelowADInplaceOrView below;
-    return handle<Tensor2(const Tensor&, const Tensor&, double, int64_t, double, double, const optional<Tensor>&)>("marl_amd::sample_logits")
-        .call(logits, u, temperature, top_k, top_p, min_p, settings);
+    return MARL_OP("sample_logits", Tensor2(const Tensor&, const Tensor&, double, int64_t, double, double, const optional<Tensor>&)).call(logits, u, temperature, top_k, top_p, min_p, settings);
 }
 
 }  // namespace
