@@ -88,7 +88,9 @@ struct Rows {
 struct On {
     c10::DeviceGuard guard;
     void* stream;
-    explicit On(const Tensor& t) : guard(t.device()), stream(c10::hip::getCurrentHIPStream(t.device().index()).stream()) {}
+    explicit On(const Tensor& t) : guard(t.device()), stream(c10::hip::getCurrentHIPStream(t.device().index()).stream()) {
+        TORCH_CHECK(lib.marl_strerror, "marl_amd: the trunk operators are not bound to libmarl_env.so (import marl_amd.ops binds them)");
+    }
 };
 
 Tensor scratch(const Tensor& like, size_t bytes) { return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)); }
