@@ -205,7 +205,7 @@ _torch_loaded = False
 
 def load_torch():
     """Register the trunk operators (torch.ops.marl_amd.gated_linear, residual_norm, keyed_dropout, sample_logits) and bind
-    them to the library that load() uses; raise if either has not been built."""
+    them to the library that load() uses; raise MarlError if either has not been built."""
     global _torch_loaded
     if _torch_loaded:
         return
@@ -214,7 +214,10 @@ def load_torch():
     if not os.path.exists(path):
         raise MarlError(f"{path} not found: build it with `python -c 'import __graft_entry__ as g; g.build()'`")
     import torch
-    torch.ops.load_library(path)
+    try:
+        torch.ops.load_library(path)
+    except OSError as e:                 # built against another torch
+        raise MarlError(f"{path} does not load ({e}): build it again") from e
     if C.CDLL(path).marl_torch_bind(os.path.abspath(LIB_PATH).encode()) != 0:
         raise MarlError(f"{LIB_PATH} lacks an entry point of the trunk operators: build it again")
     _torch_loaded = True

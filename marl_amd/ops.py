@@ -239,4 +239,27 @@ def _(state, handle, actions, noise, obs, reward, truncated):
 
 
 # -- operators of a residual policy trunk and of the draw from its head: registered by libmarl_torch.so (csrc/marl_torch.cpp) --
-_lib.load_torch()
+def _refuse_trunk_operators(reason: str):
+    """Without libmarl_torch.so the ops above work all the same; these four then say what is missing when they are called."""
+    import torch.library
+    lib = torch.library.Library("marl_amd", "FRAGMENT")
+
+    def refuse(*args, **kwargs):
+        raise _lib.MarlError(reason)
+
+    for schema in ("gated_linear(Tensor x, Tensor w_gate, Tensor w_up, str act=\"silu\") -> Tensor",
+                   "residual_norm(Tensor x, Tensor block, Tensor w_post, Tensor w_pre, Tensor? gate=None, float scale=1.0, "
+                   "float eps=1e-5, str kind=\"rms\") -> (Tensor, Tensor)",
+                   "keyed_dropout(Tensor x, float p, int seed, Tensor? keys=None) -> Tensor",
+                   "sample_logits(Tensor logits, Tensor u, float temperature=1.0, int top_k=0, float top_p=1.0, "
+                   "float min_p=0.0, *, Tensor? settings=None) -> (Tensor, Tensor)"):
+        lib.define(schema)
+        lib.impl(schema[:schema.index("(")], refuse, "CompositeImplicitAutograd")
+    return lib
+
+
+try:
+    _lib.load_torch()
+except (_lib.MarlError, AttributeError) as e:            # AttributeError: libmarl_env.so lacks a function of this version
+    if not hasattr(torch.ops.marl_amd, "gated_linear"):  # else: registered but not bound, and the operators say so
+        _refused = _refuse_trunk_operators(str(e))
