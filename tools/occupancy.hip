@@ -1,5 +1,5 @@
 // Prints what the HIP runtime says about the residency of the step kernels (workgroups per CU).
-// hipcc --offload-arch=gfx950 -O3 -ffp-contract=off -std=c++17 -Iinclude tools/occupancy.hip -o build_ab/occupancy
+// hipcc --offload-arch=gfx950 -O3 -ffp-contract=off -std=c++17 -Xclang -target-feature -Xclang -packed-fp32-ops -Iinclude tools/occupancy.hip -o build_ab/occupancy
 #include "../marl_amd/csrc/marl_env.hip"
 #include <stdio.h>
 int main() {
