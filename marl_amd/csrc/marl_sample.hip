@@ -399,12 +399,19 @@ template <int THREADS> __device__ __forceinline__ int bin_of(double z) {
     return b < (double)(BINS - 1) ? (int)b : BINS - 1;
 }
 
-// A float32 bound of the logits in bins up to `bin`: those of later bins lie below it, or so little above that the bin
-// itself has to be looked at (a step of float32 lower than the edge, for the rounding on the way).
+// Float32 bounds of the logits of a bin: none of bins up to `bin` lies below lower_edge, none of bins from `bin` on above
+// upper_edge; what else lies between them is told apart by its bin.  The slack covers the roundings on the way: to float32, of
+// the edge's size, and of the distance to the maximum, in float64, of the maximum's (which counts where the edge is next to 0).
+__device__ __forceinline__ double edge_slack(double edge, float top) { return fabs(edge) * 0x1p-22 + fabs((double)top) * 0x1p-48 + 0x1p-126; }
 template <int THREADS> __device__ __forceinline__ float lower_edge(int bin, float top, double inv_t) {
     if (bin >= Dim<THREADS>::BINS - 1) return -HUGE_VALF;
-    const float edge = (float)((double)top - (double)(bin + 1) / (Dim<THREADS>::PER_NAT * inv_t));
-    return edge - fabsf(edge) * 0x1p-22f - 0x1p-126f;
+    const double edge = (double)top - (double)(bin + 1) / (Dim<THREADS>::PER_NAT * inv_t);
+    return (float)(edge - edge_slack(edge, top));
+}
+template <int THREADS> __device__ __forceinline__ float upper_edge(int bin, float top, double inv_t) {
+    if (bin <= 0) return HUGE_VALF;
+    const double edge = (double)top - (double)bin / (Dim<THREADS>::PER_NAT * inv_t);
+    return (float)(edge + edge_slack(edge, top));
 }
 
 template <int THREADS> struct Shared {
@@ -519,8 +526,7 @@ __device__ __noinline__ Cut resolve(Shared<THREADS>& s, const T* row, int32_t V,
     // cheap bounds first: most of the row is outside of the bin (+inf logits, whose distances are not numbers: no bounds)
     const bool bounded = fabsf(top) < HUGE_VALF;
     const float floor_ = bounded ? lower_edge<THREADS>((int)bin, top, inv_t) : -HUGE_VALF;
-    const float edge = (float)((double)top - (double)bin / (Dim<THREADS>::PER_NAT * inv_t));
-    const float ceiling = bounded && bin > 0 ? edge + fabsf(edge) * 0x1p-22f + 0x1p-126f : HUGE_VALF;
+    const float ceiling = bounded ? upper_edge<THREADS>((int)bin, top, inv_t) : HUGE_VALF;
     for (;;) {
         if (threadIdx.x == 0) { s.n = 0; s.found = 0xFFFFFFFFu; s.found_count = 0; }
         __syncthreads();
