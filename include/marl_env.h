@@ -520,7 +520,8 @@ int marl_keyed_dropout(int32_t dtype, int64_t rows, int32_t d, const void *x, in
  * (0: off), top_p (1: off), min_p (0: off), in that order, then the first index, in index order, whose running weight
  * exceeds u times the sum; log_prob is that index's log-probability among what was kept.  Equal logits: lower index
  * first.  settings: NULL, or float [rows][4] = temperature, top_k, top_p, min_p of every row instead of the four scalars
- * (out-of-range values there turn the filter off; temperature <= 0 is 0).  NaN logits count as -inf; a row without any
+ * (nothing is refused there: NaN and top_k < 1 turn a filter off, temperature <= 0 is 0, top_p <= 0 keeps the first element,
+ * min_p > 1 is 1).  Weights below 2^-43 of the largest count as 0; u is clamped to [0, 1].  NaN logits count as -inf; a row without any
  * other gives index -1 and log_prob -inf.  The result is a function of the row alone (no order of adding enters). */
 int marl_sample_logits(int32_t dtype, int64_t rows, int32_t V, const void *logits, int64_t ld, const float *u,
                        float temperature, int32_t top_k, float top_p, float min_p, const float *settings, int64_t *index,

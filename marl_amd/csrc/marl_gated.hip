@@ -18,10 +18,13 @@
 // elements each, against 4 T d h operations for computing a and b again: in 16 bits da and db would be rounded twice
 // (gradients off by 0.0029 instead of 0.0024 in bf16), and p = b act'(a) may lie outside of float16 where y and the gradients
 // do not.
-// Bound by the matrix cores; FWD / DX / DW measured: T 8192, d 2048, h 8192, bf16: 621 / 465 / 472 us (885 / 1183 / 1165
-// TFLOP/s); T 32768, d 128, h 512, float32: 105 / 80 / 77 us (82 / 108 / 111); T 1999, d 1000, h 2731, float16, operands
-// packed: 50 / 36 / 37 us (436 / 601 / 592).  da and db are bandwidth: 109 us at the first sizes (6.1 TB/s).  Few rows are
-// bound by the weights' bytes: T 1, d 2048, h 8192, bf16: 13.9 us a call (4.8 TB/s).
+// Bound by the matrix cores; FWD / DX / DW measured: T 8192, d 2048, h 8192, bf16: 636 / 462 / 469 us (865 / 1190 / 1172
+// TFLOP/s; FWD without f and p 476 us: the rest is their stores, behind which a block's matrix cores idle); T 32768, d 128,
+// h 512, float32: 103 / 79 / 77 us (83 / 109 / 112); T 1999, d 1000, h 2731, float16: 54 / 36 / 36 us (404 / 601 / 605), at
+// d 1001 six copies of operands of 4.5 us each more in a step.  da and db are bandwidth: 156 us at the first sizes (6.0 TB/s).
+// Few rows are bound by the weights' bytes: T 1, d 2048, h 8192, bf16: 14.0 us a call (4.8 TB/s).  Far from any bound: forward
+// of more than 64 rows over narrow weights, whose few tiles each run all of k (T 128, d 4096, h 512: 33 us in bf16, 239 in
+// float32, where 64 rows take 27 and 25).
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -456,7 +459,7 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
         const int64_t row0 = m0 + wm * (BM / WM) + 32 * i;
         if constexpr (MODE == FWD) {
             // f and p are float32: with four columns a lane one store of theirs covers whole lines, with eight (16-bit types)
-            // every other 16 bytes of twice as many.  (The same width without them: the compiler rounds f b to float16 in one
+            // every other 16 bytes of twice as many (T 8192, d 2048, h 8192, bf16, step: 1615 and 1880 us).  (The same width without them: the compiler rounds f b to float16 in one
             // step or in two by what is around it, and y must not depend on whether f and p are kept.)
             constexpr int W = 4, PER_ROW = COLS / 2 / W;
             by_act(args.act, [&](auto kind) {
@@ -639,8 +642,9 @@ __global__ __launch_bounds__(256) void gated_da_db_kernel(const float* __restric
 // -- host ------------------------------------------------------------------------------------------------------------
 struct Plan { bool big; int slices, stages; };
 
-// Tile and split of one product.  256 x 256 tiles (one block of eight waves per CU) where they fill the chip, else
-// 128 x 128; if those are too few for that, k is cut into slices of at least sixteen stages, up to one block for every CU.
+// Tile and split of one product.  256 x 256 tiles (one block of eight waves per CU) where they fill three quarters of the
+// chip, else 128 x 128 (T 4096, d 1024, forward, large : small tiles; bf16: 128 large ones 31 : 25 us, 160 30 : 33, 192 32 : 36;
+// float32: 192 241 : 209, 224 240 : 252); if those are too few for that, k is cut into slices of at least sixteen stages, up to one block for every CU.
 // Two blocks for every CU cost more in the slices' sum than they save (kernel and sum, one : two blocks a CU; T 1999,
 // d 1000, h 2731, float16, dx and dW: 89 : 95 us; T 32768, d 128, h 512, float32, dW: 93 : 102 us).
 template <typename T> Plan plan_of(int mode, int64_t M, int64_t N, int64_t K) {
@@ -685,7 +689,9 @@ hipError_t launch_product(ProductArgs& a, float* partial, hipStream_t stream) {
     return hipGetLastError();
 }
 
-// slices of d over blocks: fewer than 64 blocks of columns, and a run for every wave of every slice
+// Slices of d over blocks: fewer than 64 blocks of columns, and a run for every wave of every slice.  (d 4096, one slice : up to
+// 128 blocks in all; bf16, T 1: 16 blocks of columns 20 : 16 us, 32 20 : 15, 48 20 : 18, 64 20 : 19, T 64: 32 32 : 23, 64 33 : 28;
+// float32, T 1: 16 50 : 17, 32 52 : 21, 48 53 : 33, 64 53 : 34.  Two slices would still gain there; from 128 blocks on there is one.)
 template <typename T> int few_rows_slices(int64_t d, int64_t h) {
     const int64_t blocks = (h + 31) / 32, most = d / (64 * Chunk<T>::n);
     if (blocks >= 64 || most < 2) return 1;

@@ -5,8 +5,8 @@
 // The kept set is always a prefix of the order, so it is described by its last element (value, index).  Weights are
 // held as integers, w 2^42 rounded: their sums do not depend on the order of adding, so LDS atomics and any launch shape
 // give the same index; sums are 64-bit integers (a row of 2^20 logits cannot overflow) or, up to 2048 logits, float64, which
-// holds integers up to 2^53 exactly.  exp is evaluated in float64: an index
-// depends on which side of a border a sum of many weights falls.
+// holds integers up to 2^53 exactly.  Weights below 2^-43 of the largest are 0: such an element is never drawn, for u = 0 or 1
+// neither.  exp is evaluated in float64: an index depends on which side of a border a sum of many weights falls.
 // NaN counts as -inf; +inf takes all the mass (several share it); a row without a finite or +inf logit gives index -1
 // and log-probability -inf.  temperature <= 0: the first largest logit.
 // Rows of up to 64 logits: a group of lanes per row, everything in registers.  Up to 2048: a wave per row, likewise; the
@@ -19,7 +19,7 @@
 // the kept.
 // Measured: 131072 x 4 float32 6.8 us; 256 x 131072 bf16 with settings per row 66 to 151 us, by whether some row's settings
 // miss the short way for a small top-k (67 MB would take 13): one row's chain of passes on one CU is the bound, as for one
-// row of 100003 (22 us).
+// row of 100003 (22 us).  65 to 2048 logits: 37 282 x 900 f16 with top-k 64 and top-p 188 us, top-p alone 234 (67 MB: 13): bisection.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -385,6 +385,12 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(const SampleArgs a) {
 // -- longer rows: a workgroup per row ----------------------------------------------------------------------------------
 // The workgroups: 1024 threads (one to a CU) for long rows if there are few, 256 for shorter rows and for many: what a row
 // takes is mostly waiting, for its loads and at barriers (981 x 34 183 f16, top-k 64 and top-p: 74 us with 1024 threads).
+// Where the two meet depends on the row's length: f16, 1024 : 256 threads, top-k 64 with top-p | top-p | no filter, us:
+//     34 183 x  256     22 :  24  |    73 :  106  |   25 :  43          131 072 x  512     67 :  57  |   298 :  366  |  106 : 158
+//     34 183 x  512     40 :  28  |   139 :  122  |   47 :  54          131 072 x 1024    124 :  89  |   590 :  549  |  202 : 254
+//     34 183 x 1024     78 :  38  |   272 :  169  |   90 :  81          262 144 x 1024    214 : 200  |  1049 : 1072  |  377 : 502
+// hence 256 from 512 rows on, up to 131 072 logits, and up to 8192 logits for any number of rows (9000 x 64: 18 : 17 | 42 : 45 |
+// 16 : 18; x 384: 33 : 18 | 90 : 53 | 30 : 22).
 // With 256, registers are held to six workgroups a CU; left free, the kernel takes more than 128 and two fit (same call,
 // two : four : six a CU: 52 : 37 : 37 us; 4096 x 3000: 116 : 65 : 52; top-p alone, where six spill, 219 : 159 : 162).
 template <int THREADS> struct Dim {

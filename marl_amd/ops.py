@@ -21,6 +21,11 @@ three are differentiable (the dropout twice, the others once), all take float32,
     keyed_dropout(x, p, seed, keys)                                 mask from (seed, row key, column), never stored
     sample_logits(logits, u, temperature, top_k, top_p, min_p)      index and log-probability of a filtered draw
 
+All tensors of a call have one type (keys, u and settings apart): torch.autocast does not cast for them, and a mixture is
+refused.  Forward-mode derivatives are refused.  temperature, top_p and min_p are taken as float32, as `settings` holds them.
+16-bit types: gated_linear rounds the gradients da and db, which are matrix operands, and every result once; what forward
+keeps is float32.  residual_norm keeps its inputs, so x must not be changed in place before backward.
+
 Bit matrices are int32 tensors [E, N, ceil(N/32)]: row i, bit j of word j // 32.
 """
 from __future__ import annotations
