@@ -1,5 +1,5 @@
-"""GPU tests of the trunk operators at sizes where a workgroup takes more than one turn of its loop over rows: rows beyond what
-the chip holds at once, with a ragged last turn."""
+"""GPU tests of the trunk operators at sizes where a workgroup takes more than one turn of its loop over rows (rows beyond what
+the chip holds at once, with a ragged last turn) or a tile takes all of a long k."""
 import pytest
 import torch
 
@@ -55,3 +55,10 @@ def test_keyed_dropout_more_groups_than_threads(T, d):
         close("dropout", got[at], want, (half_step(BF16) + 3 * U) * want.abs() + tiny(BF16))
     # every row was written, by the same rule: the mask of the gradient is that of the value
     assert torch.equal(y.detach() == 0, (g == 0) | (x.detach() == 0)) or bool(((y.detach() == 0) == (g == 0))[(x.detach() != 0) & (gy != 0)].all())
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("T,d,h", [(64, 4096, 128), (65, 4096, 128), (64, 2500, 512), (65, 2500, 512), (300, 4096, 130)])
+def test_gated_linear_narrow_weights_of_long_rows(T, d, h, dt):
+    """Both sides of the number of rows up to which k is sliced in forward."""
+    gated_check(T, d, h, dt, "silu", seed=T + h)
