@@ -16,7 +16,7 @@
 // 16-bit types: v_mfma_f32_32x32x16 with float32 accumulators; float32: v_mfma_f32_32x32x2.  da and db are rounded to
 // the element type, once, because they are matrix operands.  f and p are kept between forward and backward in float32, T h
 // elements each, against 4 T d h operations for computing a and b again: in 16 bits da and db would be rounded twice
-// (gradients off by 0.0029 instead of 0.0024 in bf16), and p = b act'(a) may lie outside of float16 where y and the gradients
+// (gradients off by 0.0029 instead of 0.0023 in bf16), and p = b act'(a) may lie outside of float16 where y and the gradients
 // do not.
 // Bound by the matrix cores; FWD / DX / DW measured: T 8192, d 2048, h 8192, bf16: 636 / 462 / 469 us (865 / 1190 / 1172
 // TFLOP/s; FWD without f and p 476 us: the rest is their stores, behind which a block's matrix cores idle); T 32768, d 128,
@@ -459,8 +459,9 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
         const int64_t row0 = m0 + wm * (BM / WM) + 32 * i;
         if constexpr (MODE == FWD) {
             // f and p are float32: with four columns a lane one store of theirs covers whole lines, with eight (16-bit types)
-            // every other 16 bytes of twice as many (T 8192, d 2048, h 8192, bf16, step: 1615 and 1880 us).  (The same width without them: the compiler rounds f b to float16 in one
-            // step or in two by what is around it, and y must not depend on whether f and p are kept.)
+            // every other 16 bytes of twice as many (T 8192, d 2048, h 8192, bf16, step: 1615 and 1880 us).  The same width
+            // where they are not kept: the compiler rounds f b to float16 in one step or in two by what is around it, and y
+            // must not depend on whether f and p are kept.
             constexpr int W = 4, PER_ROW = COLS / 2 / W;
             by_act(args.act, [&](auto kind) {
                 constexpr int ACT = decltype(kind)::value;
@@ -644,7 +645,8 @@ struct Plan { bool big; int slices, stages; };
 
 // Tile and split of one product.  256 x 256 tiles (one block of eight waves per CU) where they fill three quarters of the
 // chip, else 128 x 128 (T 4096, d 1024, forward, large : small tiles; bf16: 128 large ones 31 : 25 us, 160 30 : 33, 192 32 : 36;
-// float32: 192 241 : 209, 224 240 : 252); if those are too few for that, k is cut into slices of at least sixteen stages, up to one block for every CU.
+// float32: 192 241 : 209, 224 240 : 252); if those are too few for that, k is cut into slices of at least sixteen stages, up to
+// one block for every CU (the gradients' products only).
 // Two blocks for every CU cost more in the slices' sum than they save (kernel and sum, one : two blocks a CU; T 1999,
 // d 1000, h 2731, float16, dx and dW: 89 : 95 us; T 32768, d 128, h 512, float32, dW: 93 : 102 us).
 template <typename T> Plan plan_of(int mode, int64_t M, int64_t N, int64_t K) {

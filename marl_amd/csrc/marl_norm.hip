@@ -5,13 +5,14 @@
 //     dx = scale t,  dgate = t o,  dblock = N'(t gate w_post; block),  dw_post = sum t gate block^,  dw_pre = sum gn y^,
 //     N'(g; v) = r (g - mean(g) [layer only] - v^ mean(g v^)).
 // Bandwidth bound: a row lives in the registers of its threads (16 lanes to 1024 threads, one 16-byte chunk each up to 512
-// chunks, two or four beyond), so that forward reads x and block once and backward gy, gn, x and block once.  Workgroups stay and take
-// row after row: the next row's chunks are under way while the sums of this one cross the waves, and the weights' chunks
+// chunks, two or four beyond), so that forward reads x and block once and backward gy, gn, x and block once.  Workgroups stay
+// and take row after row: the next row's chunks are under way while the sums of this one cross the waves, and the weights' chunks
 // are held throughout.  Sums and statistics are float32; y is
 // normalised before it is rounded.  m and r of both norms are kept (16 bytes a row), and backward computes y from x and block
 // again: taken from memory, y has been rounded, and with the statistics of the unrounded row that leaves an error of half a
-// step of y, times r, in y^ (a row of mean 64 and spread 1 in bf16: 0.14), at the same bytes.  The column sums of backward stay in registers over a workgroup's rows, go to a partial row per
-// workgroup and are added by a second launch in a fixed order (no atomics: results do not vary from run to run).
+// step of y, times r, in y^ (a row of mean 64 and spread 1 in bf16: 0.14), at the same bytes.  The column sums of backward
+// stay in registers over a workgroup's rows, go to a partial row per workgroup and are added by a second launch in a fixed
+// order (no atomics: results do not vary from run to run).
 // Measured: forward 131072 x 128 float32 43 us (6.2 TB/s), 16384 x 4096 bf16 102 us (5.3); backward 80 us (5.0) and, with a
 // channel gate, 211 us (3.8) and 6 us for the columns' sum: 154 registers, three waves a SIMD.  Rows of more than 1024 chunks
 // do not fit: backward spills 35 to 326 registers a thread and is bound by that traffic (4096 x 8192 float32 473 us, 1.7 TB/s;
